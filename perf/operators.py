@@ -281,8 +281,7 @@ def _own_tree(st):
     return cast_b200.varlen_tree_attention_paged(st["q"], st["k_pages"][0], st["v_pages"][0], st["table"], st["k"],
                                                  st["v"], st["cu_q"], st["lens"], st["packs"], words,
                                                  parent=st["parent"] if words is None else None,
-                                                 max_pack=st["max_pack"], max_prefix=st["max_prefix"], out=st["out"],
-                                                 fp32_path="exact")
+                                                 max_pack=st["max_pack"], max_prefix=st["max_prefix"], out=st["out"])
 
 
 def _rotate(x, pos, inv_freq, interleaved):
