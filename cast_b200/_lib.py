@@ -32,7 +32,8 @@ EXPORTS = ("cast_strerror", "cast_version", "cast_device_error", "cast_tree_attn
            "cast_tree_attn_fwd_noalloc", "cast_tree_attn_store_fwd", "cast_tree_attn_store_workspace_size",
            "cast_tree_walk_greedy", "cast_select_global_topk", "cast_append_store", "cast_gather_cache",
            "cast_test_set_wait_limit_ns", "cast_tree_attn_workspace_size_kv", "cast_kv_ragged_gather",
-           "cast_test_set_tc_kernel")
+           "cast_test_set_tc_kernel", "cast_paged_append", "cast_paged_decode_attn",
+           "cast_paged_decode_workspace_size", "cast_tree_attn_paged_fwd", "cast_tree_attn_paged_workspace_size")
 CAST_NOALLOC_SCRATCH_BYTES = 64 << 20
 
 
@@ -132,6 +133,22 @@ def lib():
     L.cast_gather_cache.restype = c_int
     L.cast_gather_cache.argtypes = [c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_i64, c_vp, c_vp, c_int,
                                     c_vp, c_int, c_vp]
+    L.cast_paged_append.restype = c_int
+    L.cast_paged_append.argtypes = [c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_vp, c_i64, c_vp,
+                                    c_vp, c_i64, c_int, c_vp, c_int, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_int,
+                                    c_int, ctypes.c_float, c_vp, c_vp, c_int, c_vp, c_vp]
+    L.cast_paged_decode_attn.restype = c_int
+    L.cast_paged_decode_attn.argtypes = [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_i64, c_int, c_vp,
+                                         c_int, c_int, c_int, c_int, c_int, c_int, ctypes.c_float, ctypes.c_float,
+                                         c_int, c_vp, c_vp, c_sz, c_vp]
+    L.cast_paged_decode_workspace_size.restype = c_sz
+    L.cast_paged_decode_workspace_size.argtypes = [c_int] * 5
+    L.cast_tree_attn_paged_fwd.restype = c_int
+    L.cast_tree_attn_paged_fwd.argtypes = [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_i64, c_int,
+                                           c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int, c_int, c_int,
+                                           c_int, c_int, ctypes.c_float, c_int, c_int, c_vp, c_sz, c_vp]
+    L.cast_tree_attn_paged_workspace_size.restype = c_sz
+    L.cast_tree_attn_paged_workspace_size.argtypes = [c_int] * 8
     L.cast_test_set_wait_limit_ns.restype = None
     L.cast_test_set_wait_limit_ns.argtypes = [ctypes.c_uint64]
     L.cast_test_set_tc_kernel.restype = None

@@ -57,6 +57,14 @@ struct AttnParams {
   // only full 256-row blocks (pair_full_only), the single-CTA kernel only each sequence's partial
   // last block (tail_only; its grid then holds one row block per (sequence, KV head, key chunk)).
   int pair_full_only, tail_only;
+  // Paged prefix (cu_kv NULL): the prefix of sequence b is in pages [num_pages, H_kv, page_size, D],
+  // key n in row n % page_size of page page_table[b * table_stride + n / page_size]; the pack K/V are
+  // k / v as in store mode. `box` = rows of one page copy of the tensor-core kernel.
+  const void *k_pages, *v_pages;
+  int64_t pg_p, pg_h, pg_r;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int num_pages, page_size, box;
 };
 
 // Key tiles of one sequence: the whole range for the regular layout, the
@@ -145,7 +153,9 @@ __device__ __forceinline__ uint32_t visible32(const uint64_t* anc, int W, int nb
   return lim >= 32 ? bits : (lim <= 0 ? 0u : bits & ((1u << lim) - 1u));
 }
 
-template <typename T, int D>
+// PAGED = false: K/V are [total_kv, H_kv, D] rows (prefix, then pack). PAGED = true: the prefix is read
+// from its pages (one table entry per row) and the pack from the pack rows.
+template <typename T, int D, bool PAGED = false>
 __global__ void __launch_bounds__(simt::NT)
 attn_simt_kernel(const AttnParams p) {
   using namespace simt;
@@ -161,8 +171,11 @@ attn_simt_kernel(const AttnParams p) {
   const int tid = threadIdx.x;
   const int ty = tid >> 4, tx = tid & 15;
   const int b = blockIdx.y / p.H_kv, h = blockIdx.y % p.H_kv;
-  const SeqMeta m = load_seq(p.cu_q, p.cu_kv, p.prefix_len, p.pack_len, b, p.total_q, p.total_kv,
-                             p.max_pack, p.max_kv);
+  SeqMeta m;
+  if constexpr (PAGED)
+    m = load_seq_store(p.cu_q, p.prefix_len, p.pack_len, b, p.total_q, p.store_rows, p.max_pack);
+  else
+    m = load_seq(p.cu_q, p.cu_kv, p.prefix_len, p.pack_len, b, p.total_q, p.total_kv, p.max_pack, p.max_kv);
   if (!m.ok) {
     if (tid == 0 && blockIdx.x == 0 && blockIdx.z == 0) report(CAST_DEV_BAD_LAYOUT);
     return;
@@ -213,9 +226,20 @@ attn_simt_kernel(const AttnParams p) {
       const int n = kb + rr;
       float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
       if (n < k_end) {
-        const int64_t row = m.kv0 + n;
-        kx = load4<T>(K + row * p.sk_m + (int64_t)h * p.sk_h + c4);
-        vx = load4<T>(V + row * p.sv_m + (int64_t)h * p.sv_h + c4);
+        if (PAGED && n < m.S) {
+          const int page = p.page_table[b * p.table_stride + n / p.page_size];
+          if (page >= 0 && page < p.num_pages) {
+            const int64_t at = (int64_t)page * p.pg_p + (int64_t)(n % p.page_size) * p.pg_r + (int64_t)h * p.pg_h + c4;
+            kx = load4<T>(static_cast<const T*>(p.k_pages) + at);
+            vx = load4<T>(static_cast<const T*>(p.v_pages) + at);
+          } else {
+            report(CAST_DEV_BAD_LAYOUT);
+          }
+        } else {
+          const int64_t row = PAGED ? (int64_t)m.q0 + n - m.S : (int64_t)m.kv0 + n;
+          kx = load4<T>(K + row * p.sk_m + (int64_t)h * p.sk_h + c4);
+          vx = load4<T>(V + row * p.sv_m + (int64_t)h * p.sv_h + c4);
+        }
       }
       *reinterpret_cast<float4*>(sK + rr * QS + c4) = kx;
       *reinterpret_cast<float4*>(sV + rr * D + c4) = vx;
@@ -353,10 +377,8 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const AttnParams p) {
   }
   const int b = lo;
   SeqMeta m;
-  if (p.store_mode) {
-    m.q0 = p.cu_q[b]; m.kv0 = 0; m.S = p.prefix_len[b]; m.P = p.pack_len[b];
-    m.ok = m.q0 >= 0 && m.S >= 0 && m.P >= 0 && m.P <= p.max_pack && m.S <= p.store_rows &&
-           (long long)m.q0 + m.P <= p.total_q;
+  if (p.cu_kv == nullptr) {   // prefix in stores or pages
+    m = load_seq_store(p.cu_q, p.prefix_len, p.pack_len, b, p.total_q, p.store_rows, p.max_pack);
   } else {
     m = load_seq(p.cu_q, p.cu_kv, p.prefix_len, p.pack_len, b, p.total_q, p.total_kv, p.max_pack, p.max_kv);
   }

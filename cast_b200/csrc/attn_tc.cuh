@@ -127,15 +127,22 @@ __device__ __forceinline__ int ranked_sequence(const AttnParams& p, int rank, in
   return seq_of_rank;
 }
 
-// STORE = false: K/V are [total_kv, H_kv, D] (tmK, tmV; tmKp/tmVp unused).
-// STORE = true: tmK/tmV map the per-request prefix stores [B, H_kv, S_max, D]
+// kRagged: K/V are [total_kv, H_kv, D] (tmK, tmV; tmKp/tmVp unused).
+// kStore: tmK/tmV map the per-request prefix stores [B, H_kv, S_max, D]
 // (4-D), tmKp/tmVp the pack K/V [total_q, H_kv, D].
-template <bool BF16, bool STORE>
+// kPaged: as kStore with the prefix in pages [num_pages, H_kv, page_size, D]. A 128-key tile is
+// 128 / box copies per 64-column half, box = gcd(page_size, 128) rows, so every copy stays inside its
+// page (the 128-byte swizzle goes by the shared-memory address, so boxes of fewer than 8 rows land as
+// one of 128 would put them). The producer warp's lanes issue them side by side, each from a table
+// entry that it read while the previous tile was under way.
+enum KvLayout { kRagged = 0, kStore = 1, kPaged = 2 };
+template <bool BF16, int LAYOUT>
 __global__ void __launch_bounds__(NT, 1)
 attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKp,
                const __grid_constant__ CUtensorMap tmVp) {
   using namespace tc;
+  constexpr bool STORE = LAYOUT != kRagged;   // prefix tiles and pack tiles come from different tensors
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* sAnc = reinterpret_cast<uint64_t*>(smem + SMEM_ANC);
@@ -168,9 +175,8 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
   const int b = ranked_sequence(p, rank, reinterpret_cast<int*>(smem + SMEM_K));  // K ring as scratch
   SeqMeta m;
   if constexpr (STORE) {
-    m.q0 = p.cu_q[b]; m.kv0 = 0; m.S = p.prefix_len[b]; m.P = p.pack_len[b];
-    m.ok = m.q0 >= 0 && m.S >= 0 && m.P >= 0 && m.P <= p.max_pack && m.S <= p.store_rows && b < p.store_batch &&
-           (long long)m.q0 + m.P <= p.total_q;
+    m = load_seq_store(p.cu_q, p.prefix_len, p.pack_len, b, p.total_q, p.store_rows, p.max_pack);
+    m.ok = m.ok && b < p.store_batch;
   } else {
     m = load_seq(p.cu_q, p.cu_kv, p.prefix_len, p.pack_len, b, p.total_q, p.total_kv, p.max_pack, p.max_kv);
   }
@@ -265,14 +271,36 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
   const uint32_t ring = smem_u32(smem + (is_k ? SMEM_K : SMEM_V));
   const CUtensorMap* m_reg = is_k ? &tmK : &tmV;
   const CUtensorMap* m_pack = is_k ? &tmKp : &tmVp;
+  // Paged prefix: lane l copies half l & 1 of boxes l / 2, l / 2 + 16, ...; the table entry of its first
+  // box in tile j + 1 is read while tile j is being copied.
+  auto page_at = [&](int n) -> int {
+    return n < m.S ? p.page_table[b * p.table_stride + n / p.page_size] : -1;
+  };
+  int next_page = -1;
+  if (LAYOUT == kPaged && (warp == 0 || warp == 2)) next_page = page_at(t_begin * BN + (lane >> 1) * p.box);
   // one 128-key tile (two 64-column halves) into ring slot j % NST
   auto issue_tile = [&](int j) {
-    if (elect_one()) {
-      const uint32_t dst = ring + (j % NST) * TILE_BYTES, bar = smem_u32(&full[j % NST]);
+    const uint32_t dst = ring + (j % NST) * TILE_BYTES, bar = smem_u32(&full[j % NST]);
+    const int t = t_begin + j;
+    if (LAYOUT == kPaged && t < nt_pre) {
+      const int n0 = t * BN, boxes = (min(BN, m.S - n0) + p.box - 1) / p.box;
+      int page = next_page;
+      next_page = page_at(n0 + BN + (lane >> 1) * p.box);
+      if (elect_one()) mbar_expect_tx(bar, boxes * p.box * 256);
+      __syncwarp();
+      for (int i = lane >> 1; i < boxes; i += 16) {
+        const int n = n0 + i * p.box;
+        if (i >= 16) page = page_at(n);
+        if (page < 0 || page >= p.num_pages) {
+          report(CAST_DEV_BAD_LAYOUT);
+          page = p.num_pages;          // past the last page: the copy fills zeros
+        }
+        tma_load_4d(dst + (lane & 1) * HALF_BYTES + i * p.box * 128, m_reg, (lane & 1) * 64, n % p.page_size, h, page, bar);
+      }
+    } else if (elect_one()) {
       mbar_expect_tx(bar, TILE_BYTES);
       for (int hf = 0; hf < 2; ++hf) {
         if constexpr (STORE) {
-          const int t = t_begin + j;
           if (t < nt_pre) tma_load_4d(dst + hf * HALF_BYTES, m_reg, hf * 64, t * BN, h, b, bar);
           else tma_load_3d(dst + hf * HALF_BYTES, m_pack, hf * 64, h, m.q0 + (t - nt_pre) * BN, bar);
         } else {

@@ -16,6 +16,8 @@
 #include "attn_pair.cuh"
 #include "tree_build.cuh"
 #include "verify_ops.cuh"
+#include "paged_append.cuh"
+#include "paged_decode.cuh"
 
 namespace cast {
 namespace {
@@ -73,7 +75,7 @@ SimtPlan plan_simt(int B, int total_q, int H_q, int H_kv, int D, int max_pack, i
   return pl;
 }
 
-template <typename T>
+template <typename T, bool PAGED = false>
 int launch_simt(AttnParams& p, const SimtPlan& pl, cudaStream_t st) {
   p.n_split = pl.n_split;
   p.chunk = pl.chunk;
@@ -82,12 +84,12 @@ int launch_simt(AttnParams& p, const SimtPlan& pl, cudaStream_t st) {
   dim3 grid(pl.m_tiles, p.B * p.H_kv, pl.n_split);
   if (p.D == 128) {
     const size_t smem = simt::smem_bytes<128>(pl.W);
-    cudaFuncSetAttribute(attn_simt_kernel<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    attn_simt_kernel<T, 128><<<grid, simt::NT, smem, st>>>(p);
+    cudaFuncSetAttribute(attn_simt_kernel<T, 128, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    attn_simt_kernel<T, 128, PAGED><<<grid, simt::NT, smem, st>>>(p);
   } else {
     const size_t smem = simt::smem_bytes<64>(pl.W);
-    cudaFuncSetAttribute(attn_simt_kernel<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    attn_simt_kernel<T, 64><<<grid, simt::NT, smem, st>>>(p);
+    cudaFuncSetAttribute(attn_simt_kernel<T, 64, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    attn_simt_kernel<T, 64, PAGED><<<grid, simt::NT, smem, st>>>(p);
   }
   if (cudaGetLastError() != cudaSuccess) return CAST_ERR_LAUNCH;
   if (pl.n_split > 1) {
@@ -194,7 +196,22 @@ bool make_store_map(CUtensorMap* map, const void* base, int dtype, int batch, in
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool STORE>
+// 4-D map over pages [num_pages, heads, page_size, 128]: box = 64 dims x `box` rows of one head of one page.
+bool make_pages_map(CUtensorMap* map, const void* base, int dtype, int num_pages, int heads, int page_size,
+                    int64_t s_p, int64_t s_h, int64_t s_r, int box_rows) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  cuuint64_t dims[4] = {128, (cuuint64_t)page_size, (cuuint64_t)heads, (cuuint64_t)num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)s_r * 2, (cuuint64_t)s_h * 2, (cuuint64_t)s_p * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType dt = dtype == CAST_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, dt, 4, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int LAYOUT>
 int launch_tc_maps(AttnParams& p, const TcPlan& pl, int dtype, cudaStream_t st, const CUtensorMap& mq,
                    const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mkp, const CUtensorMap& mvp,
                    bool combine = true) {
@@ -209,11 +226,11 @@ int launch_tc_maps(AttnParams& p, const TcPlan& pl, int dtype, cudaStream_t st, 
   const size_t smem = tca::smem_bytes(p.G, pl.W);
   dim3 grid(p.tail_only ? 1 : pl.m_blocks, p.B * p.H_kv, pl.n_split);
   if (dtype == CAST_BF16) {
-    cudaFuncSetAttribute(tca::attn_tc_kernel<true, STORE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    tca::attn_tc_kernel<true, STORE><<<grid, tca::NT, smem, st>>>(p, mq, mk, mv, mkp, mvp);
+    cudaFuncSetAttribute(tca::attn_tc_kernel<true, LAYOUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    tca::attn_tc_kernel<true, LAYOUT><<<grid, tca::NT, smem, st>>>(p, mq, mk, mv, mkp, mvp);
   } else {
-    cudaFuncSetAttribute(tca::attn_tc_kernel<false, STORE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    tca::attn_tc_kernel<false, STORE><<<grid, tca::NT, smem, st>>>(p, mq, mk, mv, mkp, mvp);
+    cudaFuncSetAttribute(tca::attn_tc_kernel<false, LAYOUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    tca::attn_tc_kernel<false, LAYOUT><<<grid, tca::NT, smem, st>>>(p, mq, mk, mv, mkp, mvp);
   }
   if (cudaGetLastError() != cudaSuccess) return CAST_ERR_LAUNCH;
   if (combine && pl.n_split > 1) {
@@ -334,7 +351,7 @@ int launch_tc(AttnParams& p, const TcPlan& pl, int dtype, cudaStream_t st, bool 
       !make_map(&mk, p.k, dtype, p.total_kv, p.H_kv, p.sk_m, p.sk_h, 1, tca::BN) ||
       !make_map(&mv, p.v, dtype, p.total_kv, p.H_kv, p.sv_m, p.sv_h, 1, tca::BN))
     return CAST_ERR_LAUNCH;
-  return launch_tc_maps<false>(p, pl, dtype, st, mq, mk, mv, mk, mv, combine);
+  return launch_tc_maps<tca::kRagged>(p, pl, dtype, st, mq, mk, mv, mk, mv, combine);
 }
 
 // CTA-pair kernel: a cluster of two CTAs per 256-row block; K tiles arrive in 64-key halves (one
@@ -787,7 +804,7 @@ int cast_tree_attn_store_fwd(const void* q, const void* k_store, const void* v_s
       !make_map(&mkp, k_pack, dtype, total_q, H_kv, skp[0], skp[1], 1, tca::BN) ||
       !make_map(&mvp, v_pack, dtype, total_q, H_kv, svp[0], svp[1], 1, tca::BN))
     return CAST_ERR_LAUNCH;
-  return launch_tc_maps<true>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp);
+  return launch_tc_maps<tca::kStore>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp);
 }
 
 int cast_kv_ragged_gather(const void* k_store, const void* v_store, const void* k_pack, const void* v_pack,
@@ -1073,6 +1090,333 @@ int cast_gather_cache(int n_layers, const void* const* src_kv, void* const* dst_
   a.keep_stride = 0; a.cu_q = nullptr;
   return kv_gather(n_layers, src_kv, dst_kv, src_kv, (int64_t)n_prefix * a.src_sr, a, a.dst_cap,
                    static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
+
+// ---- paged key-value cache ------------------------------------------------------------------------
+
+namespace cast {
+namespace {
+
+// Pages [num_pages, H_kv, page_size, D]: strides (page, head, row) that keep every row 16-byte aligned.
+bool page_strides_ok(const int64_t* st, int elem_bytes) {
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0 || st[i] * elem_bytes % 16 != 0) return false;
+  return true;
+}
+
+template <typename T>
+cudaError_t launch_append(papp::Args& a, const papp::Layers& ly, bool vec, int nl, int64_t rows, int sms, cudaStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int v = vec ? V : 1;
+  if (a.interleaved && vec) {
+    a.X = a.D / v;
+    a.np = 0;
+  } else {
+    a.np = a.h / v;
+    a.X = a.np + (a.D - 2 * a.h) / v;
+  }
+  int64_t blocks;
+  if (a.keep) {
+    a.tok = papp::MAX_TOK;
+    blocks = a.B;
+  } else {
+    a.tok = rows * nl >= (int64_t)papp::MAX_TOK * 8 * sms ? papp::MAX_TOK : 1;
+    blocks = (rows + a.tok - 1) / a.tok;
+  }
+  const dim3 grid((unsigned)blocks, (unsigned)nl);
+  if (vec) papp::append_kernel<T, V><<<grid, papp::NT, 0, st>>>(a, ly);
+  else papp::append_kernel<T, 1><<<grid, papp::NT, 0, st>>>(a, ly);
+  return cudaGetLastError();
+}
+
+// Tile of query heads of one KV head, and the instantiation that takes it.
+int decode_rows(int dtype, int G) {
+  if (dtype == CAST_F32) return G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : 8;
+  return G <= 16 ? 16 : 32;
+}
+
+int decode_workers(int dtype, int D, int sms) {
+  const int per_sm = dtype == CAST_F32 ? (D == 128 ? pdec::ctas_per_sm<float, 128>() : pdec::ctas_per_sm<float, 64>())
+                                       : (D == 128 ? pdec::ctas_per_sm<__half, 128>() : pdec::ctas_per_sm<__half, 64>());
+  return sms * per_sm * pdec::NW;
+}
+
+// Workspace: first steps [B + 1] int64, then the partials of two pieces per worker.
+struct DecodeLayout {
+  int rows, workers;
+  size_t o, ml, total;
+};
+DecodeLayout decode_layout(int dtype, int B, int G, int D, int sms) {
+  DecodeLayout l;
+  l.rows = decode_rows(dtype, G);
+  l.workers = decode_workers(dtype, D, sms);
+  const size_t slots = 2 * (size_t)l.workers * l.rows;
+  l.o = align256((size_t)(B + 1) * sizeof(int64_t));
+  l.ml = l.o + align256(slots * D * sizeof(float));
+  l.total = l.ml + align256(slots * 2 * sizeof(float));
+  return l;
+}
+
+template <typename K>
+cudaError_t launch_decode_worker(K kern, const pdec::Params& p, size_t smem, cudaStream_t st) {
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  kern<<<p.W / pdec::NW, pdec::NT, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch_decode(const pdec::Params& p, cudaStream_t st) {
+  constexpr size_t smem = (size_t)pdec::NW * pdec::stages<T, D>() * pdec::stage_bytes<T, D>();
+  cudaError_t e;
+  if constexpr (std::is_same<T, float>::value) {
+    switch (p.rows) {
+      case 1: e = launch_decode_worker(pdec::decode_f32_kernel<D, 1>, p, smem, st); break;
+      case 2: e = launch_decode_worker(pdec::decode_f32_kernel<D, 2>, p, smem, st); break;
+      case 4: e = launch_decode_worker(pdec::decode_f32_kernel<D, 4>, p, smem, st); break;
+      default: e = launch_decode_worker(pdec::decode_f32_kernel<D, 8>, p, smem, st); break;
+    }
+  } else {
+    e = p.rows == 16 ? launch_decode_worker(pdec::decode_mma_kernel<T, D, 1>, p, smem, st)
+                     : launch_decode_worker(pdec::decode_mma_kernel<T, D, 2>, p, smem, st);
+  }
+  if (e != cudaSuccess) return e;
+  // the join may start while the last workers run; it waits for them before its first read
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(((int64_t)p.B * p.H_q + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, pdec::decode_join_kernel<T, D>, p);
+}
+
+}  // namespace
+}  // namespace cast
+
+extern "C" {
+
+int cast_paged_append(int n_layers, void* const* pages_kv, const void* const* new_kv, int dtype, int H_kv, int D,
+                      int num_pages, int page_size, const int64_t* page_strides, int64_t total,
+                      const int64_t* new_strides, const int32_t* page_table, int64_t table_stride, int max_pages,
+                      const int32_t* seq_len, int B, const int32_t* cu_q, const int32_t* keep, int keep_stride,
+                      const int32_t* accepted, const int32_t* positions, const float* inv_freq, int n_freq,
+                      int interleaved, float rope_scale, const void* q, void* q_out, int H_q,
+                      const int64_t* q_strides, cast_stream_t stream) {
+  if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return CAST_ERR_DTYPE;
+  if (n_layers < 0 || H_kv < 1 || D < 1 || num_pages < 1 || page_size < 1 || total < 0 || max_pages < 0 || B < 0 ||
+      table_stride < 0 || keep_stride < 0 || n_freq < 0 || 2 * n_freq > D)
+    return CAST_ERR_SHAPE;
+  if (D > papp::MAX_D) return CAST_ERR_HEAD_DIM;
+  if (total > 0x7fffffffLL) return CAST_ERR_SHAPE;
+  if ((q == nullptr) != (q_out == nullptr)) return CAST_ERR_NULL;
+  if (q && (n_layers != 1 || keep || H_q < 1 || n_freq == 0)) return CAST_ERR_SHAPE;
+  if ((keep == nullptr) != (accepted == nullptr) || (keep && !cu_q)) return CAST_ERR_NULL;
+  if (n_layers == 0 || B == 0 || total == 0 || (keep && keep_stride == 0)) return CAST_OK;
+  if (!pages_kv || !new_kv || !page_strides || !new_strides || !page_table || !seq_len || (n_freq > 0 && !inv_freq) ||
+      (q && !q_strides))
+    return CAST_ERR_NULL;
+  for (int i = 0; i < 2 * n_layers; ++i)
+    if (!pages_kv[i] || !new_kv[i]) return CAST_ERR_NULL;
+  if (max_pages < 1) return CAST_ERR_SHAPE;
+  const int e = dtype == CAST_F32 ? 4 : 2, v = 16 / e;
+  papp::Args a{};
+  a.H_kv = H_kv; a.H_q = q ? H_q : 0; a.D = D; a.h = n_freq;
+  a.interleaved = interleaved ? 1 : 0;
+  a.rope_scale = rope_scale;
+  a.num_pages = num_pages; a.page_size = page_size; a.max_pages = max_pages; a.B = B;
+  a.table_stride = table_stride;
+  a.pk_p = page_strides[0]; a.pk_h = page_strides[1]; a.pk_r = page_strides[2];
+  a.pv_p = page_strides[3]; a.pv_h = page_strides[4]; a.pv_r = page_strides[5];
+  a.sk_t = new_strides[0]; a.sk_h = new_strides[1]; a.sv_t = new_strides[2]; a.sv_h = new_strides[3];
+  if (q) { a.sq_t = q_strides[0]; a.sq_h = q_strides[1]; a.so_t = q_strides[2]; a.so_h = q_strides[3]; }
+  a.total = total;
+  a.table = page_table; a.seq_len = seq_len; a.cu_q = cu_q; a.keep = keep; a.accepted = accepted;
+  a.positions = positions; a.keep_stride = keep_stride; a.inv_freq = inv_freq;
+  a.q = q; a.q_out = q_out;
+  // 16-byte pieces where every head and every half of a rotated head starts on one
+  bool vec = D % v == 0 && (interleaved ? 2 * n_freq : n_freq) % v == 0;
+  for (int i = 0; i < 6; ++i) vec = vec && page_strides[i] % v == 0;
+  for (int i = 0; i < 4; ++i) vec = vec && new_strides[i] % v == 0 && (!q || q_strides[i] % v == 0);
+  vec = vec && (!q || (aligned(q, 16) && aligned(q_out, 16)));
+  for (int i = 0; i < 2 * n_layers; ++i) vec = vec && aligned(pages_kv[i], 16) && aligned(new_kv[i], 16);
+  const int sms = sm_count();
+  if (sms <= 0) return CAST_ERR_DEVICE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t rows = cu_q ? total : std::min<int64_t>(total, B);
+  for (int l0 = 0; l0 < n_layers; l0 += papp::MAXL) {
+    const int nl = std::min(papp::MAXL, n_layers - l0);
+    papp::Layers ly{};
+    for (int l = 0; l < nl; ++l)
+      for (int kv = 0; kv < 2; ++kv) {
+        ly.src[l][kv] = new_kv[2 * (l0 + l) + kv];
+        ly.dst[l][kv] = pages_kv[2 * (l0 + l) + kv];
+      }
+    cudaError_t err;
+    switch (dtype) {
+      case CAST_F32: err = launch_append<float>(a, ly, vec, nl, rows, sms, st); break;
+      case CAST_BF16: err = launch_append<__nv_bfloat16>(a, ly, vec, nl, rows, sms, st); break;
+      default: err = launch_append<__half>(a, ly, vec, nl, rows, sms, st); break;
+    }
+    if (err != cudaSuccess) return CAST_ERR_LAUNCH;
+  }
+  return CAST_OK;
+}
+
+size_t cast_paged_decode_workspace_size(int dtype, int B, int H_q, int H_kv, int D) {
+  if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return 0;
+  if (B <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || (D != 64 && D != 128)) return 0;
+  const int sms = sm_count();
+  return decode_layout(dtype, B, H_q / H_kv, D, sms > 0 ? sms : 148).total;
+}
+
+int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pages, void* out, float* lse, int dtype,
+                           const int64_t* strides, const int32_t* page_table, int64_t table_stride, int max_pages,
+                           const int32_t* seq_len, int B, int H_q, int H_kv, int D, int num_pages, int page_size,
+                           float sm_scale, float softcap, int window, const float* alibi_slopes, void* workspace,
+                           size_t workspace_bytes, cast_stream_t stream) {
+  if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return CAST_ERR_DTYPE;
+  if (B < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || num_pages < 1 || page_size < 1 || max_pages < 0 ||
+      table_stride < 0 || window < 0 || !(softcap >= 0.f))
+    return CAST_ERR_SHAPE;
+  if (D != 64 && D != 128) return CAST_ERR_HEAD_DIM;
+  if (B == 0) return CAST_OK;
+  if (!q || !k_pages || !v_pages || !out || !strides || !seq_len || (!page_table && max_pages > 0)) return CAST_ERR_NULL;
+  // strides: q (batch, head), pages (page, head, row), out (batch, head)
+  const int e = dtype == CAST_F32 ? 4 : 2;
+  for (int i : {0, 1, 5, 6})
+    if (strides[i] % 4 != 0) return CAST_ERR_ALIGN;
+  if (!page_strides_ok(strides + 2, e)) return CAST_ERR_ALIGN;
+  if (!aligned(q, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 16)) return CAST_ERR_ALIGN;
+  const int sms = sm_count();
+  if (sms <= 0) return CAST_ERR_DEVICE;
+  const int G = H_q / H_kv;
+  const DecodeLayout lay = decode_layout(dtype, B, G, D, sms);
+  if (!workspace || workspace_bytes < lay.total || !aligned(workspace, 256)) return CAST_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  pdec::Params p{};
+  p.q = q; p.k = k_pages; p.v = v_pages; p.out = out; p.lse = lse;
+  p.sq_b = strides[0]; p.sq_h = strides[1];
+  p.s_p = strides[2]; p.s_h = strides[3]; p.s_r = strides[4];
+  p.so_b = strides[5]; p.so_h = strides[6];
+  p.table = page_table; p.seq_len = seq_len; p.table_stride = table_stride;
+  p.B = B; p.H_q = H_q; p.H_kv = H_kv; p.G = G;
+  p.rows = lay.rows; p.tiles = (G + lay.rows - 1) / lay.rows;
+  p.num_pages = num_pages; p.page_size = page_size; p.max_pages = max_pages;
+  p.window = window;
+  p.scale = sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)D);
+  p.softcap = softcap;
+  p.slopes = alibi_slopes;
+  p.W = lay.workers;
+  p.cum = reinterpret_cast<int64_t*>(ws);
+  p.ws_o = reinterpret_cast<float*>(ws + lay.o);
+  p.ws_ml = reinterpret_cast<float*>(ws + lay.ml);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t err;
+  if (dtype == CAST_F32) err = D == 128 ? launch_decode<float, 128>(p, st) : launch_decode<float, 64>(p, st);
+  else if (dtype == CAST_BF16) err = D == 128 ? launch_decode<__nv_bfloat16, 128>(p, st) : launch_decode<__nv_bfloat16, 64>(p, st);
+  else err = D == 128 ? launch_decode<__half, 128>(p, st) : launch_decode<__half, 64>(p, st);
+  return err == cudaSuccess ? CAST_OK : CAST_ERR_LAUNCH;
+}
+
+size_t cast_tree_attn_paged_workspace_size(int dtype, int B, int total_q, int H_q, int H_kv, int D, int max_pack,
+                                           int max_prefix) {
+  if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return 0;
+  if (B <= 0 || total_q <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || (D != 64 && D != 128)) return 0;
+  const int sms = sm_count();
+  const size_t ws = plan_simt(B, total_q, H_q, H_kv, D, max_pack, max_prefix + max_pack, sms).ws_bytes;
+  if (dtype == CAST_F32 || D != 128 || 128 % (H_q / H_kv) != 0) return ws;
+  return std::max(ws, plan_tc_store(B, total_q, H_q, H_kv, max_pack, max_prefix, sms).ws_bytes);
+}
+
+int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_pack,
+                             const void* v_pack, void* out, int dtype, const int64_t* strides,
+                             const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cu_q,
+                             const int32_t* prefix_len, const int32_t* pack_len, const int64_t* anc_words,
+                             int anc_words_per_row, const int32_t* parent, int B, int total_q, int num_pages,
+                             int page_size, int H_q, int H_kv, int D, float sm_scale, int max_pack, int max_prefix,
+                             void* workspace, size_t workspace_bytes, cast_stream_t stream) {
+  if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return CAST_ERR_DTYPE;
+  if (B < 0 || total_q < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || max_pack < 0 || max_prefix < 0 ||
+      num_pages < 1 || page_size < 1 || max_pages < 0 || table_stride < 0 ||
+      (int64_t)max_prefix + max_pack > 0x7fffffffLL - 256)
+    return CAST_ERR_SHAPE;
+  if (D != 64 && D != 128) return CAST_ERR_HEAD_DIM;
+  if (max_pack > CAST_MAX_PACK) return CAST_ERR_PACK;
+  if (B == 0 || total_q == 0 || max_pack == 0) return CAST_OK;
+  if (!q || !k_pages || !v_pages || !k_pack || !v_pack || !out || !strides || !cu_q || !prefix_len || !pack_len ||
+      (!page_table && max_pages > 0))
+    return CAST_ERR_NULL;
+  if ((anc_words == nullptr) == (parent == nullptr)) return CAST_ERR_MASK_MODE;
+  if (anc_words && anc_words_per_row < 1) return CAST_ERR_PACK;
+  // strides: q (row, head), pages (page, head, row), k_pack, v_pack, out (row, head); dims innermost
+  const int64_t *sq = strides, *sp = strides + 2, *skp = strides + 5, *svp = strides + 7, *so = strides + 9;
+  const int e = dtype == CAST_F32 ? 4 : 2;
+  for (const int64_t* t : {sq, skp, svp, so})
+    if (t[0] % 4 != 0 || t[1] % 4 != 0) return CAST_ERR_ALIGN;
+  if (!page_strides_ok(sp, e)) return CAST_ERR_ALIGN;
+  for (const void* t : {q, k_pages, v_pages, k_pack, v_pack, (const void*)out})
+    if (!aligned(t, 16)) return CAST_ERR_ALIGN;
+  const int sms = sm_count();
+  if (sms <= 0) return CAST_ERR_DEVICE;
+  const int G = H_q / H_kv;
+  AttnParams p{};
+  p.q = q; p.k = k_pack; p.v = v_pack; p.out = out;
+  p.sq_m = sq[0]; p.sq_h = sq[1];
+  p.sk_m = skp[0]; p.sk_h = skp[1];
+  p.sv_m = svp[0]; p.sv_h = svp[1];
+  p.so_m = so[0]; p.so_h = so[1];
+  p.cu_q = cu_q; p.cu_kv = nullptr; p.prefix_len = prefix_len; p.pack_len = pack_len;
+  p.anc_words = anc_words; p.anc_wpr = anc_words_per_row; p.parent = parent;
+  p.B = B; p.total_q = total_q; p.total_kv = 0; p.H_q = H_q; p.H_kv = H_kv; p.G = G; p.D = D;
+  const float scale = sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)D);
+  p.scale_log2 = scale * kLog2e;
+  p.max_pack = max_pack; p.max_kv = max_prefix + max_pack;
+  // a prefix above max_prefix would need more key chunks than the launch has: rejected on the device
+  p.store_rows = (int)std::min<int64_t>((int64_t)max_pages * page_size, max_prefix);
+  p.store_batch = B;
+  p.k_pages = k_pages; p.v_pages = v_pages;
+  p.pg_p = sp[0]; p.pg_h = sp[1]; p.pg_r = sp[2];
+  p.page_table = page_table; p.table_stride = table_stride;
+  p.num_pages = num_pages; p.page_size = page_size;
+  p.wait_ns = g_pipeline_wait_ns.load(std::memory_order_relaxed);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  bool tensor = dtype != CAST_F32 && D == 128 && 128 % G == 0 && g_tc_kernel.load(std::memory_order_relaxed) >= 0;
+  for (const int64_t* t : {sq, skp, svp, so}) tensor = tensor && t[0] % 8 == 0 && t[1] % 8 == 0;
+  if (!tensor) {
+    const SimtPlan pl = plan_simt(B, total_q, H_q, H_kv, D, max_pack, p.max_kv, sms);
+    if (pl.ws_bytes > 0) {
+      if (!workspace || workspace_bytes < pl.ws_bytes || !aligned(workspace, 16)) return CAST_ERR_WORKSPACE;
+      p.ws_o = static_cast<float*>(workspace);
+      p.ws_ml = p.ws_o + (size_t)pl.n_split * total_q * H_q * D;
+    }
+    switch (dtype) {
+      case CAST_F32: return launch_simt<float, true>(p, pl, st);
+      case CAST_BF16: return launch_simt<__nv_bfloat16, true>(p, pl, st);
+      default: return launch_simt<__half, true>(p, pl, st);
+    }
+  }
+  p.store_mode = 1;
+  p.box = tca::BN;
+  while (page_size % p.box != 0) p.box /= 2;   // gcd(page_size, 128)
+  const TcPlan pl = plan_tc_store(B, total_q, H_q, H_kv, max_pack, max_prefix, sms);
+  if (pl.ws_bytes > 0) {
+    if (!workspace || workspace_bytes < pl.ws_bytes || !aligned(workspace, 16)) return CAST_ERR_WORKSPACE;
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_ml = p.ws_o + (size_t)pl.n_split * total_q * H_q * D;
+  }
+  CUtensorMap mq, mks, mvs, mkp, mvp;
+  if (!make_map(&mq, q, dtype, total_q, H_q, sq[0], sq[1], G, tca::BM / G) ||
+      !make_pages_map(&mks, k_pages, dtype, num_pages, H_kv, page_size, sp[0], sp[1], sp[2], p.box) ||
+      !make_pages_map(&mvs, v_pages, dtype, num_pages, H_kv, page_size, sp[0], sp[1], sp[2], p.box) ||
+      !make_map(&mkp, k_pack, dtype, total_q, H_kv, skp[0], skp[1], 1, tca::BN) ||
+      !make_map(&mvp, v_pack, dtype, total_q, H_kv, svp[0], svp[1], 1, tca::BN))
+    return CAST_ERR_LAUNCH;
+  return launch_tc_maps<tca::kPaged>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp);
 }
 
 }  // extern "C"

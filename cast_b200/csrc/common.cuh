@@ -92,4 +92,18 @@ __device__ __forceinline__ SeqMeta load_seq(const int32_t* cu_q, const int32_t* 
   return m;
 }
 
+// The same for a prefix in a per-request store or in pages (at most store_rows keys) with its own pack rows.
+__device__ __forceinline__ SeqMeta load_seq_store(const int32_t* cu_q, const int32_t* prefix_len,
+                                                  const int32_t* pack_len, int b, int total_q, int store_rows,
+                                                  int max_pack) {
+  SeqMeta m;
+  m.q0 = cu_q[b];
+  m.kv0 = 0;
+  m.S = prefix_len[b];
+  m.P = pack_len[b];
+  m.ok = m.q0 >= 0 && m.S >= 0 && m.P >= 0 && m.P <= max_pack && m.S <= store_rows &&
+         (long long)m.q0 + m.P <= total_q;
+  return m;
+}
+
 }  // namespace cast

@@ -1,0 +1,280 @@
+// Append of key / value rows to a paged cache, with the rotary position rotation on the way.
+//
+// Cache: per layer, K and V pages [num_pages, H_kv, page_size, D]; sequence b's row at slot s is row
+// s % page_size of page table[b][s / page_size]. A new row (sequence b, j-th new row) goes to slot
+// seq_len[b] + j. Its key is rotated by pos * inv_freq[i] (pos = the slot, or the caller's position):
+//   (x_a, x_b) -> (x_a cos - x_b sin, x_b cos + x_a sin),   i < h,
+// with (a, b) = (i, i + h) or (2i, 2i + 1); values from 2h on pass through. Queries beside the keys
+// turn by the same angles into q_out. The angle is formed and reduced to [-pi/4, pi/4] in 64 bits (a
+// 32-bit product is off by 0.004 rad at position 100,000), sine and cosine of the rest and the rotation
+// are 32-bit, and each result is rounded once to the cache's type.
+//
+// Bound: memory traffic for prompts (2 bytes moved per byte of k, v and q), the latency of the chain
+// length -> table entry -> store for a few rows. One CTA takes `tok` consecutive rows (4 when that still
+// gives every SM several CTAs, else 1) and all their heads, so an angle is computed once per row and
+// shared by H_q + H_kv heads through shared memory. Thread (x, y): x = 16-byte pieces of a head, y steps
+// over (row, head); a piece of the first half travels with its partner of the second half, so both
+// results come from one thread's registers. Loads are issued before the angles are computed.
+#pragma once
+
+#include "common.cuh"
+
+namespace cast {
+namespace papp {
+
+constexpr int NT = 256;
+constexpr int MAX_TOK = 4;      // rows per CTA
+constexpr int MAX_D = 256;
+constexpr int MAXL = 64;        // layers per launch
+constexpr int UNROLL = 4;       // (row, head) items a thread loads before it stores the first
+
+struct Layers {
+  const void* src[MAXL][2];   // new K, V rows
+  void* dst[MAXL][2];         // K, V pages
+};
+
+struct Args {
+  int H_kv, H_q, D, h;                 // h = rotated pairs per head
+  int interleaved, tok;
+  int X, np;                           // pieces per head and thread column count; paired pieces
+  float rope_scale;
+  int num_pages, page_size, max_pages, B;
+  int64_t table_stride;
+  int64_t pk_p, pk_h, pk_r, pv_p, pv_h, pv_r;          // page strides (elements)
+  int64_t sk_t, sk_h, sv_t, sv_h;                      // new-row strides
+  int64_t sq_t, sq_h, so_t, so_h;                      // query strides (in, out)
+  int64_t total;
+  const int32_t *table, *seq_len, *cu_q, *keep, *accepted, *positions;
+  int keep_stride;
+  const float* inv_freq;
+  const void* q;
+  void* q_out;
+};
+
+// The last b in [0, B) with cu_q[b] <= t, or -1; by one whole warp (33 samples a round).
+__device__ __forceinline__ int find_seq(const int32_t* cu_q, int B, int64_t t) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = B;
+  while (n > 32) {
+    const int step = (n + 31) / 32;
+    const int i = lane * step;
+    const int c = __popc(__ballot_sync(0xffffffffu, i < n && (int64_t)cu_q[lo + min(i, n - 1)] <= t));
+    if (c == 0) return -1;
+    lo += (c - 1) * step;
+    n = min(step, n - (c - 1) * step);
+  }
+  const int c = __popc(__ballot_sync(0xffffffffu, lane < n && (int64_t)cu_q[lo + min(lane, n - 1)] <= t));
+  return c == 0 ? -1 : lo + c - 1;
+}
+
+// cos and sin of pos * freq: quadrant and remainder in 64 bits, the remainder's functions in 32.
+__device__ __forceinline__ void cos_sin(int pos, float freq, float& c, float& s) {
+  const double th = (double)pos * (double)freq;
+  const double n = rint(th * 0.63661977236758134308);                       // 2 / pi
+  double r = fma(n, -1.57079632679489661923, th);                           // pi / 2, high part
+  r = fma(n, -6.123233995736766e-17, r);                                    // and what it leaves of pi / 2
+  float sr, cr;
+  sincosf((float)r, &sr, &cr);
+  const int k = (int)((long long)n & 3);
+  c = (k & 1) ? sr : cr;
+  s = (k & 1) ? cr : sr;
+  if (k == 1 || k == 2) c = -c;
+  if (k >= 2) s = -s;
+}
+
+// VEC consecutive elements as one memory access
+template <typename T, int VEC> struct Piece {
+  T x[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Piece<T, VEC> load_piece(const T* p) {
+  Piece<T, VEC> r;
+  if constexpr (VEC * sizeof(T) == 16) *reinterpret_cast<uint4*>(r.x) = *reinterpret_cast<const uint4*>(p);
+  else r.x[0] = *p;
+  return r;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_piece(T* p, const Piece<T, VEC>& r) {
+  if constexpr (VEC * sizeof(T) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.x);
+  else *p = r.x[0];
+}
+
+struct RowMeta {
+  int64_t row;      // source row, -1: nothing to do
+  int64_t dk, dv;   // element offset of the destination row (head 0) in the K / V pages
+  int pos;
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(NT) append_kernel(const Args a, const __grid_constant__ Layers ly) {
+  __shared__ RowMeta meta[MAX_TOK];
+  __shared__ __align__(16) float cs[MAX_TOK][MAX_D / 2], sn[MAX_TOK][MAX_D / 2];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int l = blockIdx.y;
+  const T* sk = static_cast<const T*>(ly.src[l][0]);
+  const T* sv = static_cast<const T*>(ly.src[l][1]);
+  T* dk = static_cast<T*>(ly.dst[l][0]);
+  T* dv = static_cast<T*>(ly.dst[l][1]);
+  const T* q = static_cast<const T*>(a.q);
+  T* qo = static_cast<T*>(a.q_out);
+  const int X = a.X, Y = NT / X;
+  const int x = tid % X, y = tid / X;
+  const bool half_pair = x < a.np;           // a second piece belongs to this one
+  const bool scalar_pairs = a.interleaved && VEC == 1;
+  // offsets inside a rotated head, and inside a value head
+  int off_a, off_b;
+  if (a.interleaved && VEC > 1) { off_a = x * VEC; off_b = 0; }
+  else if (scalar_pairs) { off_a = half_pair ? 2 * x : 2 * a.np + (x - a.np); off_b = 2 * x + 1; }
+  else { off_a = half_pair ? x * VEC : 2 * a.h + (x - a.np) * VEC; off_b = a.h + x * VEC; }
+  const int voff_a = x * VEC, voff_b = (X + x) * VEC;
+  const int heads = a.H_q + 2 * a.H_kv;      // H_q = 0 without queries
+  // accept mode: one CTA per sequence walks its accepted rows; else one CTA per `tok` rows
+  const bool accept = a.keep != nullptr;
+  int rounds = 1, n_acc = 0;
+  if (accept) {
+    n_acc = a.accepted[blockIdx.x];
+    if (n_acc < 0 || n_acc > a.keep_stride) {
+      if (tid == 0 && l == 0) report(CAST_DEV_BAD_LAYOUT);
+      return;
+    }
+    rounds = (n_acc + a.tok - 1) / a.tok;
+  }
+  for (int rd = 0; rd < rounds; ++rd) {
+    if (rd > 0) __syncthreads();             // the previous round's rows are done with meta, cs and sn
+    for (int k = warp; k < a.tok; k += NT / 32) {
+      int b, j;
+      int64_t row;
+      bool have;
+      if (accept) {
+        b = blockIdx.x;
+        j = rd * a.tok + k;
+        have = j < n_acc;
+        row = -1;
+        if (have) {
+          const int pk = a.keep[(int64_t)b * a.keep_stride + j];
+          const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
+          row = q0 + pk;
+          if (pk < 0 || q0 < 0 || row >= q1 || row >= a.total) {
+            if (lane == 0) report(CAST_DEV_BAD_LAYOUT);
+            have = false;
+          }
+        }
+      } else {
+        row = (int64_t)blockIdx.x * a.tok + k;
+        have = row < a.total;
+        if (a.cu_q == nullptr) {
+          b = (int)row;
+          j = 0;
+          have = have && row < a.B;
+        } else {
+          b = have ? find_seq(a.cu_q, a.B, row) : -1;
+          have = have && b >= 0;
+          j = 0;
+          if (have) {
+            const int64_t q0 = a.cu_q[b];
+            have = q0 >= 0 && row < a.cu_q[b + 1];   // rows behind the last sequence stay as they are
+            j = (int)(row - q0);
+          }
+        }
+      }
+      if (lane == 0) {
+        RowMeta m{-1, 0, 0, 0};
+        if (have) {
+          const int len = a.seq_len[b];
+          const int64_t slot = (int64_t)len + j;
+          const int64_t pi = slot / a.page_size;
+          int page = -1;
+          if (len >= 0 && pi < a.max_pages) page = a.table[(int64_t)b * a.table_stride + pi];
+          if (page < 0 || page >= a.num_pages) {
+            report(CAST_DEV_BAD_LAYOUT);
+          } else {
+            const int64_t r = slot - pi * a.page_size;
+            m.row = row;
+            m.dk = (int64_t)page * a.pk_p + r * a.pk_r;
+            m.dv = (int64_t)page * a.pv_p + r * a.pv_r;
+            m.pos = a.positions ? a.positions[row] : (int)min(slot, (int64_t)0x7fffffff);
+          }
+        }
+        meta[k] = m;
+      }
+    }
+    __syncthreads();
+    const int items = a.tok * heads;
+    bool first = true;
+    for (int i0 = y; first || i0 < items; i0 += Y * UNROLL) {
+      Piece<T, VEC> pa[UNROLL], pb[UNROLL];
+      const T* src[UNROLL];
+      if (y < Y) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          const int i = i0 + u * Y;
+          src[u] = nullptr;
+          if (i >= items) continue;
+          const int k = i / heads, hd = i - k * heads;
+          const int64_t row = meta[k].row;
+          if (row < 0) continue;
+          const bool is_v = hd >= a.H_q + a.H_kv;
+          if (hd < a.H_q) src[u] = q + row * a.sq_t + hd * a.sq_h;
+          else if (!is_v) src[u] = sk + row * a.sk_t + (hd - a.H_q) * a.sk_h;
+          else src[u] = sv + row * a.sv_t + (hd - a.H_q - a.H_kv) * a.sv_h;
+          pa[u] = load_piece<T, VEC>(src[u] + (is_v ? voff_a : off_a));
+          if (half_pair) pb[u] = load_piece<T, VEC>(src[u] + (is_v ? voff_b : off_b));
+        }
+      }
+      if (first) {
+        // the angles of this round's rows, while the first loads are under way
+        for (int e = tid; e < a.tok * a.h; e += NT) {
+          const int k = e / a.h, i = e - k * a.h;
+          if (meta[k].row < 0) continue;
+          float c, s;
+          cos_sin(meta[k].pos, a.inv_freq[i], c, s);
+          cs[k][i] = c * a.rope_scale;
+          sn[k][i] = s * a.rope_scale;
+        }
+        __syncthreads();
+        first = false;
+      }
+      if (y < Y) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          if (src[u] == nullptr) continue;
+          const int i = i0 + u * Y;
+          const int k = i / heads, hd = i - k * heads;
+          const bool is_v = hd >= a.H_q + a.H_kv;
+          T* dst;
+          if (hd < a.H_q) dst = qo + meta[k].row * a.so_t + hd * a.so_h;
+          else if (!is_v) dst = dk + meta[k].dk + (hd - a.H_q) * a.pk_h;
+          else dst = dv + meta[k].dv + (hd - a.H_q - a.H_kv) * a.pv_h;
+          if (!is_v) {
+            if (a.interleaved && VEC > 1) {
+              if (x * VEC < 2 * a.h) {
+                const float* c = cs[k] + x * (VEC / 2);
+                const float* s = sn[k] + x * (VEC / 2);
+#pragma unroll
+                for (int e = 0; e + 1 < VEC; e += 2) {
+                  const float u0 = Elem<T>::to_f(pa[u].x[e]), u1 = Elem<T>::to_f(pa[u].x[e + 1]);
+                  pa[u].x[e] = Elem<T>::from_f(u0 * c[e / 2] - u1 * s[e / 2]);
+                  pa[u].x[e + 1] = Elem<T>::from_f(u1 * c[e / 2] + u0 * s[e / 2]);
+                }
+              }
+            } else if (half_pair) {
+              const float* c = cs[k] + x * VEC;
+              const float* s = sn[k] + x * VEC;
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) {
+                const float u0 = Elem<T>::to_f(pa[u].x[e]), u1 = Elem<T>::to_f(pb[u].x[e]);
+                pa[u].x[e] = Elem<T>::from_f(u0 * c[e] - u1 * s[e]);
+                pb[u].x[e] = Elem<T>::from_f(u1 * c[e] + u0 * s[e]);
+              }
+            }
+          }
+          store_piece<T, VEC>(dst + (is_v ? voff_a : off_a), pa[u]);
+          if (half_pair) store_piece<T, VEC>(dst + (is_v ? voff_b : off_b), pb[u]);
+        }
+      }
+    }
+  }
+}
+
+}  // namespace papp
+}  // namespace cast

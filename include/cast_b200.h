@@ -13,6 +13,7 @@
  *   - cast_trees/tree.py:63-82         select_global_topk
  *   - cast_trees/serving.py:264-289    BatchedServer._append_store
  *   - cast_trees/verify.py:48-60       gather_cache
+ * and adds a paged key-value cache (append with rotation, one-token attention, tree attention).
  *
  * Conventions shared by every entry point:
  *   - All array arguments are DEVICE pointers owned by the caller. The library
@@ -393,6 +394,92 @@ int cast_append_store(int n_layers, const void* const* src_kv, void* const* dst_
 int cast_gather_cache(int n_layers, const void* const* src_kv, void* const* dst_kv, int elem_bytes, int B, int H,
                       int D, int64_t src_len, const int64_t* src_strides, const int64_t* dst_strides, int n_prefix,
                       const int32_t* keep, int n_keep, cast_stream_t stream);
+
+/*
+ * Paged key-value cache. No counterpart in the reference, whose stores are one
+ * contiguous [B, H, cap, D] tensor per layer that is copied whole when it grows or
+ * a request leaves (cast_trees/serving.py:190-205, 264-289). Per layer, keys and
+ * values are pages [num_pages, H_kv, page_size, D] (element strides for page, head
+ * and row; dim stride 1; any order of heads and rows); key n of sequence b is row
+ * n % page_size of page page_table[b * table_stride + n / page_size]. page_table
+ * rows hold max_pages int32 entries; only entries that cover a sequence's keys are
+ * read. Two sequences may share pages. A length outside [0, max_pages * page_size]
+ * or a page id outside [0, num_pages) is reported as CAST_DEV_BAD_LAYOUT and never
+ * read or written through; that sequence's results are then undefined.
+ */
+
+/*
+ * Appends new rows to every layer's pages, keys rotated on the way; the paged form
+ * of cast_append_store. pages_kv / new_kv: HOST arrays of 2 * n_layers device
+ * pointers (layer l's K at [2l], V at [2l + 1]); new rows are [total, H_kv, D].
+ * page_strides[6] = K pages (page, head, row), V pages; new_strides[4] = K (row,
+ * head), V. Which rows go where, for sequence b of length seq_len[b] before the call:
+ *   cu_q NULL:          row b to slot seq_len[b] (b < min(B, total));
+ *   cu_q [B + 1]:       rows cu_q[b] + j, j < cu_q[b + 1] - cu_q[b], to seq_len[b] + j;
+ *                       rows before cu_q[0] and from cu_q[B] on are not touched;
+ *   keep and accepted:  rows cu_q[b] + keep[b * keep_stride + j], j < accepted[b], to
+ *                       seq_len[b] + j (the lists cast_tree_walk_greedy writes).
+ * Slots written by one call must be distinct. seq_len is not changed.
+ * Rotation (n_freq > 0, 2 * n_freq <= D): pair i of a key, elements (i, i + n_freq)
+ * or, with `interleaved`, (2i, 2i + 1), turns by pos * inv_freq[i] and is multiplied
+ * by rope_scale; pos is the slot, or positions[row]. Angles are 64-bit. q [total,
+ * H_q, D] (one layer, not with keep) turns by the same angles into q_out (which may
+ * be q); q_strides[4] = q (row, head), q_out. D <= 256.
+ */
+int cast_paged_append(int n_layers, void* const* pages_kv, const void* const* new_kv, int dtype, int H_kv, int D,
+                      int num_pages, int page_size, const int64_t* page_strides, int64_t total,
+                      const int64_t* new_strides, const int32_t* page_table, int64_t table_stride, int max_pages,
+                      const int32_t* seq_len, int B, const int32_t* cu_q, const int32_t* keep, int keep_stride,
+                      const int32_t* accepted, const int32_t* positions, const float* inv_freq, int n_freq,
+                      int interleaved, float rope_scale, const void* q, void* q_out, int H_q,
+                      const int64_t* q_strides, cast_stream_t stream);
+
+/*
+ * Attention of one new token per sequence over its pages. q / out: [B, H_q, D];
+ * seq_len [B] counts the keys, the new token's own among them. Scores are
+ * q . k * sm_scale (<= 0: 1/sqrt(D)), then, where given, softcap * tanh(s / softcap)
+ * (softcap > 0), then + alibi_slopes[head] * (n - (seq_len - 1)) (float [H_q]); keys
+ * n < seq_len - window are not seen (window > 0). lse (float [B, H_q], or NULL)
+ * receives the natural log of the sum of the exponentials. A sequence without keys
+ * gives 0 and -inf. strides[7] = q (batch, head), pages (page, head, row; keys and
+ * values alike), out (batch, head); q / out strides multiples of 4 elements, page
+ * strides multiples of 16 bytes, bases 16-byte aligned. CAST_F32, CAST_BF16 or
+ * CAST_F16, D 64 or 128. The lengths are not read on the host. Two launches; the
+ * workspace (256-byte aligned, cast_paged_decode_workspace_size() bytes) needs no
+ * initial value and does not depend on the lengths.
+ */
+int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pages, void* out, float* lse, int dtype,
+                           const int64_t* strides, const int32_t* page_table, int64_t table_stride, int max_pages,
+                           const int32_t* seq_len, int B, int H_q, int H_kv, int D, int num_pages, int page_size,
+                           float sm_scale, float softcap, int window, const float* alibi_slopes, void* workspace,
+                           size_t workspace_bytes, cast_stream_t stream);
+
+/* Bytes of workspace cast_paged_decode_attn needs for these sizes (0 for sizes it does not take). */
+size_t cast_paged_decode_workspace_size(int dtype, int B, int H_q, int H_kv, int D);
+
+/*
+ * cast_tree_attn_store_fwd with the prefix in pages: sequence b's prefix keys are
+ * keys [0, prefix_len[b]) of its pages, its pack keys rows [cu_q[b], cu_q[b] +
+ * pack_len[b]) of k_pack / v_pack [total_q, H_kv, D]. Visibility, output and parent /
+ * ancestor conventions are those of cast_tree_attn_fwd. strides[11] = q (row, head),
+ * pages (page, head, row; keys and values alike), k_pack, v_pack, out (row, head);
+ * multiples of 4 elements, page strides multiples of 16 bytes, bases 16-byte aligned.
+ * CAST_BF16 / CAST_F16 with D = 128, H_q / H_kv dividing 128 and strides that are
+ * multiples of 8 run on the tensor cores, everything else (CAST_F32, exact; D = 64)
+ * on the CUDA cores. Keys past prefix_len[b] in a page are never part of the result.
+ * max_prefix bounds prefix_len[b] (a longer one is reported as CAST_DEV_BAD_LAYOUT).
+ */
+int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_pack,
+                             const void* v_pack, void* out, int dtype, const int64_t* strides,
+                             const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cu_q,
+                             const int32_t* prefix_len, const int32_t* pack_len, const int64_t* anc_words,
+                             int anc_words_per_row, const int32_t* parent, int B, int total_q, int num_pages,
+                             int page_size, int H_q, int H_kv, int D, float sm_scale, int max_pack, int max_prefix,
+                             void* workspace, size_t workspace_bytes, cast_stream_t stream);
+
+/* Bytes of workspace cast_tree_attn_paged_fwd needs for these sizes (0 is possible). */
+size_t cast_tree_attn_paged_workspace_size(int dtype, int B, int total_q, int H_q, int H_kv, int D, int max_pack,
+                                           int max_prefix);
 
 #ifdef __cplusplus
 }
