@@ -1134,7 +1134,7 @@ cudaError_t launch_append(papp::Args& a, const papp::Layers& ly, bool vec, int n
 // Tile of query heads of one KV head, and the instantiation that takes it.
 int decode_rows(int dtype, int G) {
   if (dtype == CAST_F32) return G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : 8;
-  return G <= 16 ? 16 : 32;
+  return G <= 8 ? 8 : G <= 16 ? 16 : 32;
 }
 
 int decode_workers(int dtype, int D, int sms) {
@@ -1178,14 +1178,18 @@ cudaError_t launch_decode(const pdec::Params& p, cudaStream_t st) {
       default: e = launch_decode_worker(pdec::decode_f32_kernel<D, 8>, p, smem, st); break;
     }
   } else {
-    e = p.rows == 16 ? launch_decode_worker(pdec::decode_mma_kernel<T, D, 1>, p, smem, st)
-                     : launch_decode_worker(pdec::decode_mma_kernel<T, D, 2>, p, smem, st);
+    switch (p.rows) {
+      case 8: e = launch_decode_worker(pdec::decode_mma_kernel<T, D, 1>, p, smem, st); break;
+      case 16: e = launch_decode_worker(pdec::decode_mma_kernel<T, D, 2>, p, smem, st); break;
+      default: e = launch_decode_worker(pdec::decode_mma_kernel<T, D, 4>, p, smem, st); break;
+    }
   }
   if (e != cudaSuccess) return e;
   // the join may start while the last workers run; it waits for them before its first read
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(((int64_t)p.B * p.H_q + 7) / 8));
-  cfg.blockDim = dim3(256);
+  const int per = pdec::JOIN_NT / 32 / p.join_warps;
+  cfg.gridDim = dim3((unsigned)(((int64_t)p.B * p.H_q + per - 1) / per));
+  cfg.blockDim = dim3(pdec::JOIN_NT);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1311,7 +1315,12 @@ int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pag
   p.scale = sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)D);
   p.softcap = softcap;
   p.slopes = alibi_slopes;
+  p.modified = softcap > 0.f || alibi_slopes != nullptr;
+  p.v_minus_k = static_cast<const char*>(v_pages) - static_cast<const char*>(k_pages);
   p.W = lay.workers;
+  // a unit has about W / units partials at most; eight of them are one warp's round in the join
+  p.join_warps = 1;
+  while (p.join_warps < 8 && (int64_t)p.join_warps * 8 * B * H_kv * p.tiles < p.W) p.join_warps *= 2;
   p.cum = reinterpret_cast<int64_t*>(ws);
   p.ws_o = reinterpret_cast<float*>(ws + lay.o);
   p.ws_ml = reinterpret_cast<float*>(ws + lay.ml);

@@ -14,9 +14,11 @@
 // an unnormalised partial. The join kernel (launched to overlap the tail) adds each unit's partials in
 // worker order, so results do not depend on timing; it also writes the rows that see no key (0, -inf).
 //
-// 16-bit types: scores and outputs on mma.sync m16n8k16 with the KV head's query heads as the 16 rows
-// (MT tiles of them). The loop is bound by memory, so the probabilities are carried as two 16-bit terms
-// (p = hi + lo) and the only rounding of consequence is the output's. 32-bit: FMAs on the CUDA cores.
+// 16-bit types: S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16, so that keys and head dims fill the 16
+// rows and the KV head's query heads are the 8 columns (NH tiles of them; with heads as rows a group of 4
+// left 12 of 16 rows idle and held twice the registers). The probabilities are carried as two 16-bit
+// terms (p = hi + lo): the loop is bound by memory, and the only rounding of consequence is the output's.
+// 32-bit: FMAs on the CUDA cores.
 #pragma once
 
 #include "common.cuh"
@@ -36,6 +38,7 @@ template <typename T, int D> __host__ __device__ constexpr int stages() {
   return sizeof(T) == 4 ? (D == 128 ? 3 : 6) : (D == 128 ? 3 : 6);
 }
 template <typename T, int D> __host__ __device__ constexpr int ctas_per_sm() { return sizeof(T) == 4 ? 1 : 2; }
+constexpr int JOIN_NT = 256;
 
 struct Params {
   const void *q, *k, *v;
@@ -48,6 +51,9 @@ struct Params {
   int num_pages, page_size, max_pages;
   int window;                                      // 0: none
   float scale, softcap;                            // softcap 0: none
+  int modified;                                    // softcap or slopes given
+  int64_t v_minus_k;                               // byte distance of the value pages from the key pages
+  int join_warps;                                  // warps of the join kernel per row
   const float* slopes;                             // or NULL
   int W;                                           // workers
   float* ws_o;                                     // [2 W][rows][D]
@@ -79,7 +85,10 @@ __device__ __forceinline__ int active_workers(int64_t T, int W) {
 __device__ __forceinline__ int64_t first_step(int64_t T, int n, int w) { return T * w / n; }
 __device__ __forceinline__ int worker_of(int64_t T, int n, int64_t step) { return (int)(((step + 1) * n + T - 1) / T) - 1; }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_if(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;      // 0: 16 zero bytes, nothing read
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
@@ -102,6 +111,13 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 8 x 8 16-bit matrix spread over the warp (row lane / 4, columns 2 (lane % 4) and + 1), transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // Two probabilities as hi + lo pairs of 16-bit terms.
@@ -127,10 +143,8 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A score in log2 units: scaled, capped, biased by the distance to the newest key, masked.
-__device__ __forceinline__ float score(const Params& p, float dot, int n, const Span& z, float slope) {
-  if (n < z.lo || n >= z.len) return -INFINITY;
-  float s = dot * p.scale;
+// A scaled score with its cap and its bias by the distance to the newest key, in log2 units.
+__device__ __forceinline__ float modified_score(const Params& p, float s, int n, const Span& z, float slope) {
   if (p.softcap > 0.f) s = p.softcap * tanhf(s / p.softcap);
   if (p.slopes != nullptr) s = fmaf(slope, (float)(n - (z.len - 1)), s);
   return s * kLog2e;
@@ -146,16 +160,18 @@ struct Cursor {
   int b, u, s;      // sequence, unit of the sequence (KV head x tile), step
   Span z;
 };
-__device__ __forceinline__ void advance(const Params& p, Cursor& c) {
-  if (++c.s < c.z.s1) return;
+// To the next step; true when it starts another unit.
+__device__ __forceinline__ bool advance(const Params& p, Cursor& c) {
+  if (++c.s < c.z.s1) return false;
   if (++c.u == p.H_kv * p.tiles) {
     c.u = 0;
     do {
-      if (++c.b >= p.B) return;
+      if (++c.b >= p.B) return true;
       c.z = span_of(p, c.b);
     } while (c.z.s1 <= c.z.s0);
   }
   c.s = c.z.s0;
+  return true;
 }
 
 // First step of every sequence: the block sums its threads' runs of sequences, scans the sums and finds
@@ -224,220 +240,296 @@ __device__ __forceinline__ Plan plan_steps(const Params& p, int w, Cursor& c, in
   return pl;
 }
 
-// Copies one step's keys and values into a stage: rows of D elements, 16-byte pieces permuted by the row
-// (piece c of row r at c ^ (r & 7)) so that row-wise and piece-wise reads meet all banks.
-// The caller passes this lane's key's page (lane & 15), fetched a step earlier.
+// The copying side of a worker: its own cursor, ahead of the computing one, and the page of its step,
+// read from the table while the step before it is being copied.
+// A stage holds KS rows of keys, then of values; 16-byte piece c of row r is kept at c ^ (r & 7), so that
+// row-wise and piece-wise reads meet all banks.
 template <typename T, int D>
-__device__ __forceinline__ void issue_step(const Params& p, const Cursor& c, int page, uint32_t stage) {
-  constexpr int CH = D * (int)sizeof(T) / 16;      // pieces per row
-  const int lane = threadIdx.x & 31;
-  const int n = c.s * KS + (lane & 15);
-  int64_t off = -1;
-  if (n >= c.z.lo && n < c.z.len) {
-    if (page >= 0 && page < p.num_pages) off = (int64_t)page * p.s_p + (int64_t)(n % p.page_size) * p.s_r + (int64_t)(c.u / p.tiles) * p.s_h;
-    else report(CAST_DEV_BAD_LAYOUT);
+struct Copier {
+  static constexpr int CH = D * (int)sizeof(T) / 16;      // pieces per row
+  static constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;   // rows per warp-wide copy
+  static constexpr int IT = KS * CH / 32;                 // copies per step (keys or values)
+  static constexpr int ROW = D * (int)sizeof(T);
+  Cursor c;
+  int page;               // page_size % KS == 0: the step's page; else the page of key lane & 15
+  int pi, pr;             // page_size % KS == 0: page index and first row of the step
+  const char* head;       // keys of the unit's KV head
+
+  __device__ __forceinline__ void enter(const Params& p) {
+    head = static_cast<const char*>(p.k) + (int64_t)(c.u / p.tiles) * p.s_h * (int)sizeof(T);
+    if (p.page_size % KS == 0) {
+      const int n0 = c.s * KS;
+      pi = n0 / p.page_size;
+      pr = n0 - pi * p.page_size;
+    }
   }
-  constexpr int IT = KS * CH / 32;
-  const T* k = static_cast<const T*>(p.k);
-  const T* v = static_cast<const T*>(p.v);
+  __device__ __forceinline__ void fetch(const Params& p) {
+    const int32_t* row = p.table + (int64_t)c.b * p.table_stride;
+    if (p.page_size % KS == 0) {
+      page = row[pi];
+    } else {
+      const int n = c.s * KS + (threadIdx.x & 15);
+      page = (n >= c.z.lo && n < c.z.len) ? row[n / p.page_size] : -1;
+    }
+  }
+  __device__ __forceinline__ void start(const Params& p, const Cursor& at) {
+    c = at;
+    enter(p);
+    fetch(p);
+  }
+  __device__ __forceinline__ void next(const Params& p) {
+    if (advance(p, c)) {
+      enter(p);
+    } else if (p.page_size % KS == 0) {
+      pr += KS;
+      if (pr == p.page_size) {
+        pr = 0;
+        ++pi;
+      }
+    }
+    fetch(p);
+  }
+  __device__ __forceinline__ void copy(const Params& p, uint32_t stage) const {
+    const int lane = threadIdx.x & 31;
+    const int ch = lane % CH, r0 = lane / CH;
+    const int lo = c.z.lo - c.s * KS, hi = c.z.len - c.s * KS;     // visible rows of the step: [lo, hi)
+    if (p.page_size % KS == 0) {
+      const bool ok = page >= 0 && page < p.num_pages;
+      if (!ok) report(CAST_DEV_BAD_LAYOUT);
+      const int64_t step = p.s_r * (int)sizeof(T) * RPI;
+      const char* src = head + ((int64_t)(ok ? page : 0) * p.s_p + (int64_t)(pr + r0) * p.s_r) * (int)sizeof(T) + ch * 16;
+      if (ok && lo <= 0 && hi >= KS) {
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int e = i * 32 + lane;
-    const int r = e / CH, ch = e % CH;
-    const int64_t o = __shfl_sync(0xffffffffu, off, r);
-    const bool ok = o >= 0;
-    const int64_t src = (ok ? o : 0) + ch * (16 / (int)sizeof(T));
-    const uint32_t dst = stage + r * (D * (int)sizeof(T)) + ((ch ^ (r & 7)) * 16);
-    cp16(dst, k + src, ok);
-    cp16(dst + KS * D * (int)sizeof(T), v + src, ok);
+        for (int i = 0; i < IT; ++i) {
+          const int r = i * RPI + r0;
+          const uint32_t dst = stage + r * ROW + ((ch ^ (r & 7)) * 16);
+          cp16(dst, src);
+          cp16(dst + KS * ROW, src + p.v_minus_k);
+          src += step;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+          const int r = i * RPI + r0;
+          const uint32_t dst = stage + r * ROW + ((ch ^ (r & 7)) * 16);
+          const bool in = ok && r >= lo && r < hi;
+          cp16_if(dst, in ? src : head, in);
+          cp16_if(dst + KS * ROW, (in ? src : head) + p.v_minus_k, in);
+          src += step;
+        }
+      }
+    } else {
+      const int n = c.s * KS + (lane & 15);
+      int64_t off = -1;
+      if (n >= c.z.lo && n < c.z.len) {
+        if (page >= 0 && page < p.num_pages)
+          off = ((int64_t)page * p.s_p + (int64_t)(n % p.page_size) * p.s_r) * (int)sizeof(T);
+        else
+          report(CAST_DEV_BAD_LAYOUT);
+      }
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int r = i * RPI + r0;
+        const int64_t o = __shfl_sync(0xffffffffu, off, r);
+        const char* src = head + (o >= 0 ? o : 0) + ch * 16;
+        const uint32_t dst = stage + r * ROW + ((ch ^ (r & 7)) * 16);
+        cp16_if(dst, src, o >= 0);
+        cp16_if(dst + KS * ROW, src + p.v_minus_k, o >= 0);
+      }
+    }
   }
-}
-__device__ __forceinline__ int page_of(const Params& p, const Cursor& c) {
-  const int n = c.s * KS + (threadIdx.x & 15);
-  if (c.b >= p.B || n < c.z.lo || n >= c.z.len) return -1;
-  return p.table[(int64_t)c.b * p.table_stride + n / p.page_size];
-}
+};
 
 // ---------------------------------------------------------------------------------------- 16-bit types
-template <typename T, int D, int MT>
+// NH tiles of 8 query heads of one KV head. Thread (g = lane / 4, t = lane % 4) holds the scores of keys
+// g and g + 8 and the outputs of dims 16 j + g and + 8, for heads 2t and 2t + 1 of each tile.
+template <typename T, int D, int NH>
 __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int NST = stages<T, D>(), SB = stage_bytes<T, D>();
+  constexpr int NST = stages<T, D>(), SB = stage_bytes<T, D>(), ROW = D * 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const int w = blockIdx.x * NW + warp;
   Cursor cc;
-  int64_t at = 0, end = 0;
-  const Plan pl = plan_steps(p, w, cc, at, end);
+  int64_t begin = 0, end = 0;
+  const Plan pl = plan_steps(p, w, cc, begin, end);
   if (w >= pl.n) return;
   const uint32_t ring = tc::smem_u32(smem) + warp * NST * SB;
-  const int64_t begin = at;
-  Cursor ci = cc;                      // where the copies are
-  int64_t issued = at;
-  int page = page_of(p, ci);
+  int left = (int)(end - begin);       // steps to compute
+  int to_copy = left;
+  Copier<T, D> cp;
+  cp.start(p, cc);
+  uint32_t put = ring, take = ring;    // the stages of the next copy and of the next step
   auto issue = [&]() {
-    if (issued < end) {
-      issue_step<T, D>(p, ci, page, ring + (int)((issued - begin) % NST) * SB);
-      ++issued;
-      if (issued < end) {
-        advance(p, ci);
-        page = page_of(p, ci);
-      }
+    if (to_copy > 0) {
+      cp.copy(p, put);
+      if (--to_copy > 0) cp.next(p);
+      put = put + SB == ring + NST * SB ? ring : put + SB;
     }
     cp_commit();
   };
   for (int i = 0; i < NST - 1; ++i) issue();
 
-  uint32_t qf[MT][D / 16][4];
-  float o[MT][D / 8][4], m[MT][2], l[MT][2], slope[MT][2];
+  // ldmatrix row addresses within a stage: keys as the rows of A (matrices: keys 0-7 and 8-15 of piece 2k,
+  // then of piece 2k + 1), values transposed (matrices: pieces 2j and 2j + 1 of keys 0-7, then of keys 8-15)
+  const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, kx = (lane >> 4) ^ (kr & 7);
+  const int vr = (lane & 7) + (lane >> 4) * 8, vx = ((lane >> 3) & 1) ^ (vr & 7);
+  const uint32_t koff = kr * ROW, voff = KS * ROW + vr * ROW;
+  const float c = p.scale * kLog2e;
+
+  uint32_t qf[NH][D / 16][2];
+  float o[NH][D / 16][4], m[NH][2], l[NH][2], slope[NH][2];
   bool fresh = true;                   // the next step starts a piece of a unit
   bool whole = false;                  // that piece starts at the unit's first step
   int slot = 2 * w;
-  int h = 0, h0 = 0, nrow = 0;
-  for (; at < end; ++at) {
+  int h0 = 0, nrow = 0;
+  for (; left > 0; --left) {
     if (fresh) {
       fresh = false;
       whole = cc.s == cc.z.s0;
-      h = cc.u / p.tiles;
-      h0 = h * p.G + (cc.u % p.tiles) * p.rows;
+      const int h = cc.u / p.tiles;
+      h0 = h * p.G + (cc.u - h * p.tiles) * p.rows;
       nrow = min(p.rows, h * p.G + p.G - h0);
       const T* q = static_cast<const T*>(p.q) + (int64_t)cc.b * p.sq_b + (int64_t)h0 * p.sq_h;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+      for (int a = 0; a < NH; ++a) {
+        const int r = a * 8 + g;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = mt * 16 + g + (i & 1) * 8;
-            qf[mt][k][i] = r < nrow ? *reinterpret_cast<const uint32_t*>(q + (int64_t)r * p.sq_h + k * 16 + t * 2 + (i >> 1) * 8) : 0u;
-          }
+          for (int i = 0; i < 2; ++i)
+            qf[a][k][i] = r < nrow ? *reinterpret_cast<const uint32_t*>(q + (int64_t)r * p.sq_h + k * 16 + t * 2 + i * 8) : 0u;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          m[mt][i] = -INFINITY;
-          l[mt][i] = 0.f;
-          const int r = mt * 16 + g + i * 8;
-          slope[mt][i] = (p.slopes != nullptr && r < nrow) ? p.slopes[h0 + r] : 0.f;
+          m[a][i] = -INFINITY;
+          l[a][i] = 0.f;
+          const int hr = a * 8 + t * 2 + i;
+          slope[a][i] = (p.slopes != nullptr && hr < nrow) ? p.slopes[h0 + hr] : 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j)
+        for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[mt][j][i] = 0.f;
+          for (int i = 0; i < 4; ++i) o[a][j][i] = 0.f;
       }
     }
     cp_wait<NST - 2>();
     __syncwarp();
-    const uint32_t sk = ring + (int)((at - begin) % NST) * SB, sv = sk + KS * D * (int)sizeof(T);
-    issue();                        // into the stage that the previous step left
+    const uint32_t st = take;
+    take = take + SB == ring + NST * SB ? ring : take + SB;
+    issue();                           // into the stage that the previous step left
 
-    float s[MT][2][4];
+    float s[NH][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int a = 0; a < NH; ++a)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int i = 0; i < 4; ++i) s[a][i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[mt][j][i] = 0.f;
-    {
-      const int r = (lane & 7) + (lane >> 4) * 8;   // matrices 0, 1: keys 0-7; 2, 3: keys 8-15
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t ka[4];
+      ldsm4(st + koff + ((kx ^ (2 * k)) * 16), ka);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        uint32_t b[4];
-        const int ch = 2 * k + ((lane >> 3) & 1);
-        ldsm4(sk + r * (D * 2) + ((ch ^ (r & 7)) * 16), b);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma16816<T>(s[mt][0], qf[mt][k], b[0], b[1]);
-          mma16816<T>(s[mt][1], qf[mt][k], b[2], b[3]);
-        }
-      }
+      for (int a = 0; a < NH; ++a) mma16816<T>(s[a], ka, qf[a][k][0], qf[a][k][1]);
     }
-    const int n0 = cc.s * KS;
-    uint32_t ph[MT][4], plo[MT][4];
+    const int n0 = cc.s * KS + g;
+    if (p.modified) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float mx[2] = {-INFINITY, -INFINITY};
+      for (int a = 0; a < NH; ++a)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+        for (int i = 0; i < 4; ++i)
+          s[a][i] = modified_score(p, s[a][i] * p.scale, n0 + (i >> 1) * 8, cc.z, slope[a][i & 1]);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[mt][j][i] = score(p, s[mt][j][i], n0 + j * 8 + t * 2 + (i & 1), cc.z, slope[mt][i >> 1]);
-          mx[i >> 1] = fmaxf(mx[i >> 1], s[mt][j][i]);
-        }
-      float al[2];
+      for (int a = 0; a < NH; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[a][i] *= c;
+    }
+    if (n0 - g < cc.z.lo || n0 - g + KS > cc.z.len) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (n0 + i * 8 < cc.z.lo || n0 + i * 8 >= cc.z.len)
+#pragma unroll
+          for (int a = 0; a < NH; ++a) s[a][2 * i] = s[a][2 * i + 1] = -INFINITY;
+    }
+    uint32_t ph[NH][2], pl_[NH][2];
+#pragma unroll
+    for (int a = 0; a < NH; ++a) {
+      float al[2], mu[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        const float mn = fmaxf(m[mt][i], mx[i]);
-        al[i] = mn == -INFINITY ? 1.f : ex2(m[mt][i] - mn);
-        m[mt][i] = mn;
-        l[mt][i] *= al[i];
+        float mx = fmaxf(s[a][i], s[a][2 + i]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mn = fmaxf(m[a][i], mx);
+        mu[i] = mn == -INFINITY ? 0.f : mn;
+        al[i] = ex2(m[a][i] - mu[i]);
+        m[a][i] = mn;
       }
       if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+        l[a][0] *= al[0];
+        l[a][1] *= al[1];
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-          o[mt][j][0] *= al[0]; o[mt][j][1] *= al[0];
-          o[mt][j][2] *= al[1]; o[mt][j][3] *= al[1];
+        for (int j = 0; j < D / 16; ++j) {
+          o[a][j][0] *= al[0]; o[a][j][1] *= al[1];
+          o[a][j][2] *= al[0]; o[a][j][3] *= al[1];
         }
       }
-      const float mu[2] = {m[mt][0] == -INFINITY ? 0.f : m[mt][0], m[mt][1] == -INFINITY ? 0.f : m[mt][1]};
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float p0 = ex2(s[mt][j][2 * i] - mu[i]), p1 = ex2(s[mt][j][2 * i + 1] - mu[i]);
-          l[mt][i] += p0 + p1;
-          split2<T>(p0, p1, ph[mt][j * 2 + i], plo[mt][j * 2 + i]);
-        }
+      for (int i = 0; i < 2; ++i) {
+        const float p0 = ex2(s[a][2 * i] - mu[0]), p1 = ex2(s[a][2 * i + 1] - mu[1]);
+        l[a][0] += p0;
+        l[a][1] += p1;
+        split2<T>(p0, p1, ph[a][i], pl_[a][i]);
+        ph[a][i] = transpose8(ph[a][i]);
+        pl_[a][i] = transpose8(pl_[a][i]);
+      }
     }
-    {
-      const int r = (lane & 7) + ((lane >> 3) & 1) * 8;   // matrices 0, 2: keys 0-7; 1, 3: keys 8-15
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        uint32_t b[4];
-        const int ch = 2 * j + (lane >> 4);
-        ldsm4t(sv + r * (D * 2) + ((ch ^ (r & 7)) * 16), b);
+    for (int j = 0; j < D / 16; ++j) {
+      uint32_t va[4];
+      ldsm4t(st + voff + ((vx ^ (2 * j)) * 16), va);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma16816<T>(o[mt][2 * j], ph[mt], b[0], b[1]);
-          mma16816<T>(o[mt][2 * j + 1], ph[mt], b[2], b[3]);
-          mma16816<T>(o[mt][2 * j], plo[mt], b[0], b[1]);
-          mma16816<T>(o[mt][2 * j + 1], plo[mt], b[2], b[3]);
-        }
+      for (int a = 0; a < NH; ++a) {
+        mma16816<T>(o[a][j], va, ph[a][0], ph[a][1]);
+        mma16816<T>(o[a][j], va, pl_[a][0], pl_[a][1]);
       }
     }
     const bool unit_end = cc.s + 1 == cc.z.s1;
-    if (unit_end || at + 1 == end) {
+    if (unit_end || left == 1) {
       const bool direct = whole && unit_end;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int a = 0; a < NH; ++a)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float lt = l[mt][i] + __shfl_xor_sync(0xffffffffu, l[mt][i], 1);
-          lt += __shfl_xor_sync(0xffffffffu, lt, 2);
-          const int r = mt * 16 + g + i * 8;
+          float lt = l[a][i] + __shfl_xor_sync(0xffffffffu, l[a][i], 4);
+          lt += __shfl_xor_sync(0xffffffffu, lt, 8);
+          lt += __shfl_xor_sync(0xffffffffu, lt, 16);
+          const int r = a * 8 + t * 2 + i;
           if (r >= nrow) continue;
           if (direct) {
             const float inv = lt == 0.f ? 0.f : 1.f / lt;
-            T* out = static_cast<T*>(p.out) + (int64_t)cc.b * p.so_b + (int64_t)(h0 + r) * p.so_h + t * 2;
+            T* out = static_cast<T*>(p.out) + (int64_t)cc.b * p.so_b + (int64_t)(h0 + r) * p.so_h + g;
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j) {
-              T y[2] = {Elem<T>::from_f(o[mt][j][2 * i] * inv), Elem<T>::from_f(o[mt][j][2 * i + 1] * inv)};
-              *reinterpret_cast<uint32_t*>(out + j * 8) = *reinterpret_cast<const uint32_t*>(y);
+            for (int j = 0; j < D / 16; ++j) {
+              out[j * 16] = Elem<T>::from_f(o[a][j][i] * inv);
+              out[j * 16 + 8] = Elem<T>::from_f(o[a][j][2 + i] * inv);
             }
-            if (p.lse != nullptr && t == 0)
-              p.lse[(int64_t)cc.b * p.H_q + h0 + r] = lse_of(m[mt][i], lt);
+            if (p.lse != nullptr && g == 0) p.lse[(int64_t)cc.b * p.H_q + h0 + r] = lse_of(m[a][i], lt);
           } else {
-            float* wo = p.ws_o + ((int64_t)slot * p.rows + r) * D + t * 2;
+            float* wo = p.ws_o + ((int64_t)slot * p.rows + r) * D + g;
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(wo + j * 8) = make_float2(o[mt][j][2 * i], o[mt][j][2 * i + 1]);
-            if (t == 0) *reinterpret_cast<float2*>(p.ws_ml + ((int64_t)slot * p.rows + r) * 2) = make_float2(m[mt][i], lt);
+            for (int j = 0; j < D / 16; ++j) {
+              wo[j * 16] = o[a][j][i];
+              wo[j * 16 + 8] = o[a][j][2 + i];
+            }
+            if (g == 0) *reinterpret_cast<float2*>(p.ws_ml + ((int64_t)slot * p.rows + r) * 2) = make_float2(m[a][i], lt);
           }
         }
       slot = 2 * w + 1;
       fresh = true;
     }
-    if (at + 1 < end) advance(p, cc);
+    if (left > 1) advance(p, cc);
   }
   cp_wait<0>();
 }
@@ -456,23 +548,20 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int w = blockIdx.x * NW + warp;
   Cursor cc;
-  int64_t at = 0, end = 0;
-  const Plan pl = plan_steps(p, w, cc, at, end);
+  int64_t begin = 0, end = 0;
+  const Plan pl = plan_steps(p, w, cc, begin, end);
   if (w >= pl.n) return;
   uint8_t* ring_p = smem + (size_t)warp * NST * SB;
   const uint32_t ring = tc::smem_u32(ring_p);
-  const int64_t begin = at;
-  Cursor ci = cc;
-  int64_t issued = at;
-  int page = page_of(p, ci);
+  int left = (int)(end - begin), to_copy = left;
+  Copier<float, D> cp;
+  cp.start(p, cc);
+  uint32_t put = 0, take = 0;
   auto issue = [&]() {
-    if (issued < end) {
-      issue_step<float, D>(p, ci, page, ring + (int)((issued - begin) % NST) * SB);
-      ++issued;
-      if (issued < end) {
-        advance(p, ci);
-        page = page_of(p, ci);
-      }
+    if (to_copy > 0) {
+      cp.copy(p, ring + put);
+      if (--to_copy > 0) cp.next(p);
+      put = put + SB == NST * SB ? 0 : put + SB;
     }
     cp_commit();
   };
@@ -482,7 +571,8 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
   bool fresh = true, whole = false;
   int slot = 2 * w, h0 = 0, nrow = 0;
   const int key = lane & 15, half = lane >> 4;
-  for (; at < end; ++at) {
+  const float c = p.scale * kLog2e;
+  for (; left > 0; --left) {
     if (fresh) {
       fresh = false;
       whole = cc.s == cc.z.s0;
@@ -503,15 +593,16 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
     }
     cp_wait<NST - 2>();
     __syncwarp();
-    const uint8_t* st = ring_p + (int)((at - begin) % NST) * SB;
+    const uint8_t* st = ring_p + take;
+    take = take + SB == NST * SB ? 0 : take + SB;
     issue();
 
     float s[GT];
 #pragma unroll
     for (int a = 0; a < GT; ++a) s[a] = 0.f;
 #pragma unroll 4
-    for (int c = 0; c < D / 8; ++c) {
-      const int ch = half * (D / 8) + c;
+    for (int i = 0; i < D / 8; ++i) {
+      const int ch = half * (D / 8) + i;
       const float4 x = *reinterpret_cast<const float4*>(st + key * (D * 4) + ((ch ^ (key & 7)) * 16));
 #pragma unroll
       for (int a = 0; a < GT; ++a) {
@@ -526,7 +617,8 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
 #pragma unroll
     for (int a = 0; a < GT; ++a) {
       s[a] += __shfl_xor_sync(0xffffffffu, s[a], 16);
-      s[a] = score(p, s[a], n, cc.z, slope[a]);
+      s[a] = p.modified ? modified_score(p, s[a] * p.scale, n, cc.z, slope[a]) : s[a] * c;
+      if (n < cc.z.lo || n >= cc.z.len) s[a] = -INFINITY;
       float mx = s[a];
 #pragma unroll
       for (int i = 1; i < 16; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
@@ -566,7 +658,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
       }
     }
     const bool unit_end = cc.s + 1 == cc.z.s1;
-    if (unit_end || at + 1 == end) {
+    if (unit_end || left == 1) {
       const bool direct = whole && unit_end;
 #pragma unroll
       for (int a = 0; a < GT; ++a) {
@@ -592,61 +684,110 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
       fresh = true;
     }
     __syncwarp();
-    if (at + 1 < end) advance(p, cc);
+    if (left > 1) advance(p, cc);
   }
   cp_wait<0>();
 }
 
 // ---------------------------------------------------------------------------------------- join
-// One warp per (sequence, query head): adds the partials of the row's unit, in worker order. Units that
-// one worker took whole are already written; rows without a visible key become 0 (lse -inf).
+// Adds the partials of each (sequence, query head), in worker order: join_warps warps take every
+// join_warps-th one of a row's partials, eight at a time (their sums and outputs are loaded together),
+// and the first adds up the warps' results. Units that one worker took whole are already written; rows
+// without a visible key become 0 (lse -inf).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) decode_join_kernel(const Params p) {
+__global__ void __launch_bounds__(JOIN_NT) decode_join_kernel(const Params p) {
+  constexpr int DV = D / 32, NB = 8;
+  __shared__ float part[JOIN_NT / 32][D];
+  __shared__ float2 part_ml[JOIN_NT / 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= (int64_t)p.B * p.H_q) return;
-  const int b = (int)(row / p.H_q), hq = (int)(row % p.H_q);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int jw = p.join_warps, sub = warp % jw;
+  const int64_t row = (int64_t)blockIdx.x * (JOIN_NT / 32 / jw) + warp / jw;
+  const bool have = row < (int64_t)p.B * p.H_q;
+  const int b = have ? (int)(row / p.H_q) : 0, hq = have ? (int)(row % p.H_q) : 0;
   const int64_t T_all = p.cum[p.B];
   const int64_t c0 = p.cum[b], c1 = p.cum[b + 1];
   const int units = p.H_kv * p.tiles;
   T* out = static_cast<T*>(p.out) + (int64_t)b * p.so_b + (int64_t)hq * p.so_h;
-  constexpr int DV = D / 32;
-  if (c1 == c0) {
-#pragma unroll
-    for (int i = 0; i < DV; ++i) out[lane * DV + i] = Elem<T>::from_f(0.f);
-    if (p.lse != nullptr && lane == 0) p.lse[row] = -INFINITY;
-    return;
+  int w0 = 0, w1 = 0, first = 0, r = 0;
+  const bool split = have && c1 != c0;
+  if (split) {
+    const int64_t steps = (c1 - c0) / units;
+    const int hr = hq % p.G, u = (hq / p.G) * p.tiles + hr / p.rows;
+    r = hr % p.rows;
+    const int64_t us = c0 + u * steps;
+    const int n = active_workers(T_all, p.W);
+    w0 = worker_of(T_all, n, us);
+    w1 = worker_of(T_all, n, us + steps - 1);
+    first = 2 * w0 + (first_step(T_all, n, w0) == us ? 0 : 1);
   }
-  const int64_t steps = (c1 - c0) / units;
-  const int u = (hq / p.G) * p.tiles + (hq % p.G) / p.rows, r = (hq % p.G) % p.rows;
-  const int64_t us = c0 + u * steps;
-  const int n = active_workers(T_all, p.W);
-  const int w0 = worker_of(T_all, n, us), w1 = worker_of(T_all, n, us + steps - 1);
-  if (w0 == w1) return;
-  const int first = 2 * w0 + (first_step(T_all, n, w0) == us ? 0 : 1);
-  auto slot_of = [&](int w) { return (int64_t)(w == w0 ? first : 2 * w) * p.rows + r; };
-  float M = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, p.ws_ml[slot_of(w) * 2]);
-#pragma unroll
-  for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
-  const float mu = M == -INFINITY ? 0.f : M;
-  float L = 0.f, acc[DV];
+  float M = -INFINITY, L = 0.f, acc[DV];
 #pragma unroll
   for (int i = 0; i < DV; ++i) acc[i] = 0.f;
-#pragma unroll 8
-  for (int w = w0; w <= w1; ++w) {
-    const int64_t sl = slot_of(w);
-    const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + sl * 2);
-    const float f = exp2f(ml.x - mu);
-    L = fmaf(f, ml.y, L);
-    const float* o = p.ws_o + sl * D + lane * DV;
+  if (split && w0 < w1) {
+    for (int wb = w0 + sub; wb <= w1; wb += jw * NB) {
+      float2 ml[NB];
+      float x[NB][DV];
 #pragma unroll
-    for (int i = 0; i < DV; ++i) acc[i] = fmaf(f, o[i], acc[i]);
+      for (int k = 0; k < NB; ++k) {
+        const int w = wb + k * jw;
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (w <= w1) {
+          const int64_t sl = (int64_t)(w == w0 ? first : 2 * w) * p.rows + r;
+          ml[k] = *reinterpret_cast<const float2*>(p.ws_ml + sl * 2);
+          if constexpr (DV == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(p.ws_o + sl * D + lane * 4);
+          else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(p.ws_o + sl * D + lane * 2);
+        } else {
+#pragma unroll
+          for (int i = 0; i < DV; ++i) x[k][i] = 0.f;
+        }
+      }
+      float mn = M;
+#pragma unroll
+      for (int k = 0; k < NB; ++k) mn = fmaxf(mn, ml[k].x);
+      const float mu = mn == -INFINITY ? 0.f : mn, al = exp2f(M - mu);
+      L *= al;
+#pragma unroll
+      for (int i = 0; i < DV; ++i) acc[i] *= al;
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const float f = exp2f(ml[k].x - mu);
+        L = fmaf(f, ml[k].y, L);
+#pragma unroll
+        for (int i = 0; i < DV; ++i) acc[i] = fmaf(f, x[k][i], acc[i]);
+      }
+      M = mn;
+    }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  if (jw > 1) {
 #pragma unroll
-  for (int i = 0; i < DV; ++i) out[lane * DV + i] = Elem<T>::from_f(acc[i] * inv);
+    for (int i = 0; i < DV; ++i) part[warp][lane * DV + i] = acc[i];
+    if (lane == 0) part_ml[warp] = make_float2(M, L);
+    __syncthreads();
+    if (sub != 0) return;
+    float mn = M;
+    for (int k = 1; k < jw; ++k) mn = fmaxf(mn, part_ml[warp + k].x);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    float f = exp2f(M - mu);
+    L *= f;
+#pragma unroll
+    for (int i = 0; i < DV; ++i) acc[i] *= f;
+    for (int k = 1; k < jw; ++k) {
+      f = exp2f(part_ml[warp + k].x - mu);
+      L = fmaf(f, part_ml[warp + k].y, L);
+#pragma unroll
+      for (int i = 0; i < DV; ++i) acc[i] = fmaf(f, part[warp + k][lane * DV + i], acc[i]);
+    }
+    M = mn;
+  }
+  if (!have || (split && w0 == w1)) return;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T y[DV];
+#pragma unroll
+  for (int i = 0; i < DV; ++i) y[i] = Elem<T>::from_f(acc[i] * inv);
+  if constexpr (DV * sizeof(T) == 16) *reinterpret_cast<uint4*>(out + lane * DV) = *reinterpret_cast<const uint4*>(y);
+  else if constexpr (DV * sizeof(T) == 8) *reinterpret_cast<uint2*>(out + lane * DV) = *reinterpret_cast<const uint2*>(y);
+  else *reinterpret_cast<uint32_t*>(out + lane * DV) = *reinterpret_cast<const uint32_t*>(y);
   if (p.lse != nullptr && lane == 0) p.lse[row] = lse_of(M, L);
 }
 

@@ -21,7 +21,6 @@ and a verify round of draft trees, whose accepted rows are appended for every la
 A length or page id out of range is skipped on the device and reported by ``_lib.device_error()``.
 """
 import ctypes
-import math
 
 import torch
 
@@ -29,50 +28,64 @@ from . import _lib
 from .tree_attn import _DTYPES, _kernel_ready, _prep
 
 
-def _launch(dev, fn, name, *args):
-    """Calls a C entry point on dev's current stream (its last argument), with dev current."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        code = fn(*args, stream)
+# The device and the stream of a call as plain integers: the objects of torch.cuda.current_stream() take 2 us a call,
+# a tenth of what a one-token step has.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _launch(index, fn, name, *args):
+    """Calls a C entry point on the current stream of device `index` (its last argument), with that device current."""
+    if torch.cuda.current_device() == index:
+        code = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            code = fn(*args, stream)
+        with torch.cuda.device(index):
+            code = fn(*args, _raw_stream(index))
     if code:
         _lib.check(code, name)
 
 
-def _i32(t, dev, what, shape=None):
+def _i32(t, dev, what, n=None):
+    """t as a contiguous int32 tensor on dev; n: the entries it must have."""
     if not isinstance(t, torch.Tensor):
         t = torch.as_tensor(t)
     if t.dtype is not torch.int32 or t.device != dev or not t.is_contiguous():
         t = t.to(device=dev, dtype=torch.int32).contiguous()
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{what} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if n is not None and t.numel() != n:
+        raise ValueError(f"{what} must have {n} entries, not {tuple(t.shape)}")
     return t
 
 
 def _table(page_table, dev):
-    if page_table.dim() != 2:
-        raise ValueError("page_table must be [B, pages of a sequence]")
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+        raise ValueError("page_table must be a tensor [B, pages of a sequence]")
     if page_table.dtype is not torch.int32 or page_table.device != dev or page_table.stride(1) != 1:
         page_table = page_table.to(device=dev, dtype=torch.int32).contiguous()
     return page_table
 
 
 def _pages(k_pages, v_pages, name):
-    """The checked pages of one layer: [num_pages, H_kv, page_size, D], K and V alike."""
+    """Checks the pages of one layer: [num_pages, H_kv, page_size, D], K and V alike. Returns what they share."""
     if not k_pages.is_cuda:
         raise RuntimeError(f"cast_b200.{name} needs CUDA tensors (no CPU path)")
-    if k_pages.dim() != 4 or k_pages.stride(3) != 1 or k_pages.dtype not in _DTYPES:
+    shape, stride, dtype, dev = k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.device
+    if len(shape) != 4 or stride[3] != 1 or dtype not in _DTYPES:
         raise ValueError(f"{name}: pages are [num_pages, H_kv, page_size, D] of float32, bfloat16 or float16, "
                          "dim stride 1")
-    if v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride() or v_pages.dtype != k_pages.dtype \
-            or v_pages.device != k_pages.device:
+    if v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype is not dtype or v_pages.device != dev:
         raise ValueError(f"{name}: K and V pages need one shape, one dtype, one device and the same strides")
+    return shape, stride, dtype, dev
 
 
-def _ptrs(ks, vs):
-    return (ctypes.c_void_p * (2 * len(ks)))(*[t.data_ptr() for kv in zip(ks, vs) for t in kv])
+def _workspace(workspace, n, dev):
+    """The caller's workspace where it is large enough and on dev, else a new one (None: nothing is needed)."""
+    if n == 0:
+        return None
+    if workspace is None or workspace.nbytes < n or workspace.data_ptr() % 256 or workspace.device != dev:
+        return torch.empty(n, dtype=torch.uint8, device=dev)
+    return workspace
+
+
+_I4, _I6, _I7, _I11 = (ctypes.c_int64 * n for n in (4, 6, 7, 11))
 
 
 def append_paged(k_pages, v_pages, page_table, seq_len, k, v, cu_q=None, *, keep=None, accepted=None, inv_freq=None,
@@ -93,72 +106,75 @@ def append_paged(k_pages, v_pages, page_table, seq_len, k, v, cu_q=None, *, keep
     """
     many = isinstance(k_pages, (list, tuple))
     kps, vps, ks, vs = (k_pages, v_pages, k, v) if many else ((k_pages,), (v_pages,), (k,), (v,))
-    if not len(kps) == len(vps) == len(ks) == len(vs):
+    n = len(kps)
+    if not n == len(vps) == len(ks) == len(vs):
         raise ValueError("append_paged: one K and one V of pages and of new rows per layer")
-    if len(kps) == 0:
+    if n == 0:
         return None
-    kp, k0, v0 = kps[0], ks[0], vs[0]
-    for a, b in zip(kps, vps):
-        _pages(a, b, "append_paged")
-        if a is not kp and (a.shape != kp.shape or a.stride() != kp.stride() or a.dtype != kp.dtype or a.device != kp.device):
+    shape, sp, dtype, dev = _pages(kps[0], vps[0], "append_paged")
+    num_pages, H, ps, D = shape
+    rows, sk, sv = ks[0].shape, ks[0].stride(), vs[0].stride()
+    if len(rows) != 3 or rows[1] != H or rows[2] != D or sk[2] != 1 or sv[2] != 1:
+        raise ValueError("append_paged: new rows are [total, H_kv, D] of the pages' dtype and device, dim stride 1")
+    pages, new = [], []
+    for i in range(n):
+        kp, vp, a, b = kps[i], vps[i], ks[i], vs[i]
+        if i and (kp.shape != shape or vp.shape != shape or kp.stride() != sp or vp.stride() != sp
+                  or kp.dtype is not dtype or vp.dtype is not dtype or kp.device != dev or vp.device != dev):
             raise ValueError("append_paged: every layer's pages need one shape, one dtype and the same strides")
-    num_pages, H, ps, D = kp.shape
-    dev = kp.device
-    for t in (*ks, *vs):
-        if t.dim() != 3 or t.shape != k0.shape or t.shape[1] != H or t.shape[2] != D or t.dtype != kp.dtype \
-                or t.device != dev or t.stride(2) != 1:
+        if a.shape != rows or b.shape != rows or a.dtype is not dtype or b.dtype is not dtype or a.device != dev \
+                or b.device != dev:
             raise ValueError("append_paged: new rows are [total, H_kv, D] of the pages' dtype and device, dim stride 1")
-    for a, b in zip(ks, vs):
-        if a.stride() != k0.stride() or b.stride() != v0.stride():
+        if i and (a.stride() != sk or b.stride() != sv):
             raise ValueError("append_paged: every layer's new rows need the same strides")
-    total = k0.shape[0]
+        pages += (kp.data_ptr(), vp.data_ptr())
+        new += (a.data_ptr(), b.data_ptr())
+    total = rows[0]
     table = _table(page_table, dev)
-    B = table.shape[0]
-    seq_len = _i32(seq_len, dev, "seq_len", (B,))
+    B, width = table.shape
+    seq_len = _i32(seq_len, dev, "seq_len", B)
+    p_cu = p_keep = p_acc = p_pos = p_freq = p_q = p_qo = qs = None
+    w = n_freq = Hq = 0
     if cu_q is not None:
-        cu_q = _i32(cu_q, dev, "cu_q", (B + 1,))
-    if (keep is None) != (accepted is None) or (keep is not None and cu_q is None):
-        raise ValueError("append_paged: keep, accepted and cu_q go together")
-    w = 0
-    if keep is not None:
+        cu_q = _i32(cu_q, dev, "cu_q", B + 1)
+        p_cu = cu_q.data_ptr()
+    if keep is not None or accepted is not None:
+        if keep is None or accepted is None or cu_q is None:
+            raise ValueError("append_paged: keep, accepted and cu_q go together")
         keep = _i32(keep, dev, "keep")
-        accepted = _i32(accepted, dev, "accepted", (B,))
+        accepted = _i32(accepted, dev, "accepted", B)
         if keep.dim() != 2 or keep.shape[0] != B:
             raise ValueError("append_paged: keep must be [B, w]")
-        w = keep.shape[1]
-    n_freq = 0
+        w, p_keep, p_acc = keep.shape[1], keep.data_ptr(), accepted.data_ptr()
     if inv_freq is not None:
         if inv_freq.dtype is not torch.float32 or inv_freq.device != dev or not inv_freq.is_contiguous():
             inv_freq = inv_freq.to(device=dev, dtype=torch.float32).contiguous()
         n_freq = inv_freq.numel()
+        p_freq = inv_freq.data_ptr()
         if 2 * n_freq > D:
             raise ValueError("append_paged: inv_freq has more pairs than half a head")
     if positions is not None:
-        positions = _i32(positions, dev, "positions", (total,))
-    qs, Hq = None, 0
+        positions = _i32(positions, dev, "positions", total)
+        p_pos = positions.data_ptr()
     if q is not None:
-        if many or keep is not None or n_freq == 0:
+        if n > 1 or keep is not None or n_freq == 0:
             raise ValueError("append_paged: q goes with one layer and inv_freq, and not with keep")
-        if q.dim() != 3 or q.shape[0] != total or q.shape[2] != D or q.dtype != kp.dtype or q.device != dev \
-                or q.stride(2) != 1:
+        s, shape_q = q.stride(), q.shape
+        if len(shape_q) != 3 or shape_q[0] != total or shape_q[2] != D or q.dtype is not dtype or q.device != dev or s[2] != 1:
             raise ValueError("append_paged: q must be [total, H_q, D] of the pages' dtype and device, dim stride 1")
         if q_out is None:
             q_out = torch.empty_like(q)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != dev or q_out.stride(2) != 1:
+        o = q_out.stride()
+        if q_out.shape != shape_q or q_out.dtype is not dtype or q_out.device != dev or o[2] != 1:
             raise ValueError("append_paged: q_out must be like q, dim stride 1")
-        Hq = q.shape[1]
-        s, o = q.stride(), q_out.stride()
-        qs = (ctypes.c_int64 * 4)(s[0], s[1], o[0], o[1])
+        Hq, p_q, p_qo, qs = shape_q[1], q.data_ptr(), q_out.data_ptr(), _I4(s[0], s[1], o[0], o[1])
     elif q_out is not None:
         raise ValueError("append_paged: q_out without q")
-    sp, sk, sv = kp.stride(), k0.stride(), v0.stride()
-    _launch(dev, _lib.lib().cast_paged_append, "cast_paged_append", len(kps), _ptrs(kps, vps), _ptrs(ks, vs),
-            _DTYPES[kp.dtype], H, D, num_pages, ps, (ctypes.c_int64 * 6)(*sp[:3], *sp[:3]), total,
-            (ctypes.c_int64 * 4)(sk[0], sk[1], sv[0], sv[1]), table.data_ptr(), table.stride(0), table.shape[1],
-            seq_len.data_ptr(), B, None if cu_q is None else cu_q.data_ptr(), None if keep is None else keep.data_ptr(),
-            w, None if accepted is None else accepted.data_ptr(), None if positions is None else positions.data_ptr(),
-            inv_freq.data_ptr() if n_freq else None, n_freq, 1 if interleaved else 0, float(rope_scale),
-            None if q is None else q.data_ptr(), None if q is None else q_out.data_ptr(), Hq, qs)
+    ptrs = ctypes.c_void_p * (2 * n)
+    _launch(dev.index, _lib.lib().cast_paged_append, "cast_paged_append", n, ptrs(*pages), ptrs(*new), _DTYPES[dtype], H,
+            D, num_pages, ps, _I6(sp[0], sp[1], sp[2], sp[0], sp[1], sp[2]), total, _I4(sk[0], sk[1], sv[0], sv[1]),
+            table.data_ptr(), table.stride(0), width, seq_len.data_ptr(), B, p_cu, p_keep, w, p_acc, p_pos, p_freq,
+            n_freq, interleaved, rope_scale, p_q, p_qo, Hq, qs)
     return q_out
 
 
@@ -178,43 +194,44 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     float32, bfloat16 or float16, D 64 or 128, any H_q / H_kv. The key ranges of all sequences are split evenly
     over the GPU, whatever their lengths; results do not depend on timing.
     """
-    _pages(k_pages, v_pages, "decode_attention_paged")
-    dev = k_pages.device
-    num_pages, H_kv, ps, D = k_pages.shape
-    if q.dim() != 3 or q.shape[2] != D or q.dtype != k_pages.dtype or q.device != dev:
+    (num_pages, H_kv, ps, D), sp, dtype, dev = _pages(k_pages, v_pages, "decode_attention_paged")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D or q.dtype is not dtype or q.device != dev:
         raise ValueError("decode_attention_paged: q must be [B, H_q, D] of the pages' dtype and device")
-    B, H_q, _ = q.shape
+    B, H_q, _ = shape
     assert H_q % H_kv == 0
     table = _table(page_table, dev)
-    seq_len = _i32(seq_len, dev, "seq_len", (B,))
-    if table.shape[0] != B:
+    rows, width = table.shape
+    if rows != B:
         raise ValueError("decode_attention_paged: page_table must have one row per sequence")
+    seq_len = _i32(seq_len, dev, "seq_len", B)
     if window < 0 or not softcap >= 0.0:
         raise ValueError("decode_attention_paged: window and softcap must not be negative")
     q = _prep(q)
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not _kernel_ready(out):
+    elif out.shape != shape or out.dtype is not dtype or out.device != dev or not _kernel_ready(out):
         raise ValueError("out must be like q: dim stride 1, row/head strides multiple of 4, 16-byte aligned base")
+    p_slopes = p_lse = None
     if alibi_slopes is not None:
         if alibi_slopes.dtype is not torch.float32 or alibi_slopes.device != dev or not alibi_slopes.is_contiguous():
             alibi_slopes = alibi_slopes.to(device=dev, dtype=torch.float32).contiguous()
         if alibi_slopes.shape != (H_q,):
             raise ValueError("alibi_slopes must be [H_q]")
-    if lse is not None and (lse.shape != (B, H_q) or lse.dtype is not torch.float32 or lse.device != dev
-                            or not lse.is_contiguous()):
-        raise ValueError("lse must be a contiguous float32 [B, H_q]")
-    L, code = _lib.lib(), _DTYPES[q.dtype]
+        p_slopes = alibi_slopes.data_ptr()
+    if lse is not None:
+        if lse.shape != (B, H_q) or lse.dtype is not torch.float32 or lse.device != dev or not lse.is_contiguous():
+            raise ValueError("lse must be a contiguous float32 [B, H_q]")
+        p_lse = lse.data_ptr()
+    L, code = _lib.lib(), _DTYPES[dtype]
     n = L.cast_paged_decode_workspace_size(code, B, H_q, H_kv, D)
-    if workspace is None or workspace.numel() * workspace.element_size() < n or workspace.data_ptr() % 256:
-        workspace = torch.empty(n, dtype=torch.uint8, device=dev)
-    sq, sp, so = q.stride(), k_pages.stride(), out.stride()
-    _launch(dev, L.cast_paged_decode_attn, "cast_paged_decode_attn", q.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), code,
-            (ctypes.c_int64 * 7)(sq[0], sq[1], sp[0], sp[1], sp[2], so[0], so[1]), table.data_ptr(), table.stride(0),
-            table.shape[1], seq_len.data_ptr(), B, H_q, H_kv, D, num_pages, ps,
-            0.0 if sm_scale is None else float(sm_scale), float(softcap), int(window),
-            None if alibi_slopes is None else alibi_slopes.data_ptr(), workspace.data_ptr(), n)
+    workspace = _workspace(workspace, n, dev)
+    sq, so = q.stride(), out.stride()
+    _launch(dev.index, L.cast_paged_decode_attn, "cast_paged_decode_attn", q.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), out.data_ptr(), p_lse, code, _I7(sq[0], sq[1], sp[0], sp[1], sp[2], so[0], so[1]),
+            table.data_ptr(), table.stride(0), width, seq_len.data_ptr(), B, H_q, H_kv, D, num_pages, ps,
+            0.0 if sm_scale is None else sm_scale, softcap, window, p_slopes,
+            None if workspace is None else workspace.data_ptr(), n)
     return out
 
 
@@ -229,20 +246,20 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
     straight from the pages, whatever their size; float32 and other head shapes on the exact CUDA-core kernel.
     max_pack / max_prefix bound pack_len and prefix_len; given, the call reads nothing back to the host.
     """
-    _pages(k_pages, v_pages, "varlen_tree_attention_paged")
-    dev = k_pages.device
-    num_pages, H_kv, ps, D = k_pages.shape
-    total_q, H_q, _ = q.shape
+    (num_pages, H_kv, ps, D), sp, dtype, dev = _pages(k_pages, v_pages, "varlen_tree_attention_paged")
+    shape = q.shape
+    total_q, H_q, _ = shape
     assert H_q % H_kv == 0
-    for t, h in ((q, H_q), (k_pack, H_kv), (v_pack, H_kv)):
-        if t.shape != (total_q, h, D) or t.dtype != k_pages.dtype or t.device != dev:
-            raise ValueError("q must be [total_q, H_q, D] and the packs [total_q, H_kv, D], of the pages' dtype and device")
+    if shape[2] != D or k_pack.shape != (total_q, H_kv, D) or v_pack.shape != k_pack.shape or q.dtype is not dtype \
+            or k_pack.dtype is not dtype or v_pack.dtype is not dtype or q.device != dev or k_pack.device != dev \
+            or v_pack.device != dev:
+        raise ValueError("q must be [total_q, H_q, D] and the packs [total_q, H_kv, D], of the pages' dtype and device")
     if (ancestor_mask is None) == (parent is None):
         raise ValueError("pass exactly one of ancestor_mask and parent")
     table = _table(page_table, dev)
-    B = table.shape[0]
-    cu_q = _i32(cu_q, dev, "cu_q", (B + 1,))
-    prefix_len, pack_len = _i32(prefix_len, dev, "prefix_len", (B,)), _i32(pack_len, dev, "pack_len", (B,))
+    B, width = table.shape
+    cu_q = _i32(cu_q, dev, "cu_q", B + 1)
+    prefix_len, pack_len = _i32(prefix_len, dev, "prefix_len", B), _i32(pack_len, dev, "pack_len", B)
     if max_pack is None:
         max_pack = int(pack_len.max().item()) if B > 0 else 0
     if max_prefix is None:
@@ -250,25 +267,28 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
     q, k_pack, v_pack = _prep(q), _prep(k_pack), _prep(v_pack)
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not _kernel_ready(out):
+    elif out.shape != shape or out.dtype is not dtype or out.device != dev or not _kernel_ready(out):
         raise ValueError("out must be like q: dim stride 1, row/head strides multiple of 4, 16-byte aligned base")
     anc_ptr, wpr, par_ptr = None, 0, None
     if ancestor_mask is not None:
-        anc = torch.as_tensor(ancestor_mask, device=dev).to(torch.int64).reshape(total_q, -1).contiguous()
-        anc_ptr, wpr = anc.data_ptr(), anc.shape[1]
+        anc = ancestor_mask
+        if not isinstance(anc, torch.Tensor) or anc.dtype is not torch.int64 or anc.device != dev or not anc.is_contiguous():
+            anc = torch.as_tensor(anc, device=dev).to(torch.int64).contiguous()
+        wpr = anc.numel() // max(total_q, 1)
+        if anc.numel() != wpr * total_q:
+            raise ValueError("ancestor_mask must be [total_q] or [total_q, words]")
+        anc_ptr = anc.data_ptr()
     else:
-        par = _i32(parent, dev, "parent", (total_q,))
-        par_ptr = par.data_ptr()
-    L, code = _lib.lib(), _DTYPES[q.dtype]
+        parent = _i32(parent, dev, "parent", total_q)
+        par_ptr = parent.data_ptr()
+    L, code = _lib.lib(), _DTYPES[dtype]
     n = L.cast_tree_attn_paged_workspace_size(code, B, total_q, H_q, H_kv, D, max_pack, max_prefix)
-    if n > 0 and (workspace is None or workspace.numel() * workspace.element_size() < n or workspace.data_ptr() % 256):
-        workspace = torch.empty(n, dtype=torch.uint8, device=dev)
-    sq, sp, sk, sv, so = q.stride(), k_pages.stride(), k_pack.stride(), v_pack.stride(), out.stride()
-    _launch(dev, L.cast_tree_attn_paged_fwd, "cast_tree_attn_paged_fwd", q.data_ptr(), k_pages.data_ptr(),
+    workspace = _workspace(workspace, n, dev)
+    sq, sk, sv, so = q.stride(), k_pack.stride(), v_pack.stride(), out.stride()
+    _launch(dev.index, L.cast_tree_attn_paged_fwd, "cast_tree_attn_paged_fwd", q.data_ptr(), k_pages.data_ptr(),
             v_pages.data_ptr(), k_pack.data_ptr(), v_pack.data_ptr(), out.data_ptr(), code,
-            (ctypes.c_int64 * 11)(sq[0], sq[1], sp[0], sp[1], sp[2], sk[0], sk[1], sv[0], sv[1], so[0], so[1]),
-            table.data_ptr(), table.stride(0), table.shape[1], cu_q.data_ptr(), prefix_len.data_ptr(),
-            pack_len.data_ptr(), anc_ptr, wpr, par_ptr, B, total_q, num_pages, ps, H_q, H_kv, D,
-            0.0 if sm_scale is None else float(sm_scale), int(max_pack), int(max_prefix),
-            workspace.data_ptr() if n > 0 else None, n)
+            _I11(sq[0], sq[1], sp[0], sp[1], sp[2], sk[0], sk[1], sv[0], sv[1], so[0], so[1]), table.data_ptr(),
+            table.stride(0), width, cu_q.data_ptr(), prefix_len.data_ptr(), pack_len.data_ptr(), anc_ptr, wpr, par_ptr,
+            B, total_q, num_pages, ps, H_q, H_kv, D, 0.0 if sm_scale is None else sm_scale, max_pack, max_prefix,
+            None if workspace is None else workspace.data_ptr(), n)
     return out
