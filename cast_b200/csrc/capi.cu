@@ -1131,10 +1131,9 @@ cudaError_t launch_append(papp::Args& a, const papp::Layers& ly, bool vec, int n
   return cudaGetLastError();
 }
 
-// Tile of query heads of one KV head, and the instantiation that takes it.
+// Query heads of one KV head that a worker takes together.
 int decode_rows(int dtype, int G) {
-  if (dtype == CAST_F32) return G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : 8;
-  return G <= 8 ? 8 : G <= 16 ? 16 : 32;
+  return std::min(G, dtype == CAST_F32 ? 8 : 32);
 }
 
 int decode_workers(int dtype, int D, int sms) {
@@ -1143,7 +1142,7 @@ int decode_workers(int dtype, int D, int sms) {
   return sms * per_sm * pdec::NW;
 }
 
-// Workspace: first steps [B + 1] int64, then the partials of two pieces per worker.
+// Workspace: first steps [B + 1] int64, then the partials of two units per piece of the step list.
 struct DecodeLayout {
   int rows, workers;
   size_t o, ml, total;
@@ -1152,7 +1151,7 @@ DecodeLayout decode_layout(int dtype, int B, int G, int D, int sms) {
   DecodeLayout l;
   l.rows = decode_rows(dtype, G);
   l.workers = decode_workers(dtype, D, sms);
-  const size_t slots = 2 * (size_t)l.workers * l.rows;
+  const size_t slots = 2 * (size_t)l.workers * (1 + pdec::NS) * l.rows;
   l.o = align256((size_t)(B + 1) * sizeof(int64_t));
   l.ml = l.o + align256(slots * D * sizeof(float));
   l.total = l.ml + align256(slots * 2 * sizeof(float));
@@ -1162,7 +1161,7 @@ DecodeLayout decode_layout(int dtype, int B, int G, int D, int sms) {
 template <typename K>
 cudaError_t launch_decode_worker(K kern, const pdec::Params& p, size_t smem, cudaStream_t st) {
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  kern<<<p.W / pdec::NW, pdec::NT, smem, st>>>(p);
+  kern<<<p.W / pdec::NW * (1 + p.ns), pdec::NT, smem, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -1171,18 +1170,14 @@ cudaError_t launch_decode(const pdec::Params& p, cudaStream_t st) {
   constexpr size_t smem = (size_t)pdec::NW * pdec::stages<T, D>() * pdec::stage_bytes<T, D>();
   cudaError_t e;
   if constexpr (std::is_same<T, float>::value) {
-    switch (p.rows) {
-      case 1: e = launch_decode_worker(pdec::decode_f32_kernel<D, 1>, p, smem, st); break;
-      case 2: e = launch_decode_worker(pdec::decode_f32_kernel<D, 2>, p, smem, st); break;
-      case 4: e = launch_decode_worker(pdec::decode_f32_kernel<D, 4>, p, smem, st); break;
-      default: e = launch_decode_worker(pdec::decode_f32_kernel<D, 8>, p, smem, st); break;
-    }
+    if (p.rows <= 1) e = launch_decode_worker(pdec::decode_f32_kernel<D, 1>, p, smem, st);
+    else if (p.rows <= 2) e = launch_decode_worker(pdec::decode_f32_kernel<D, 2>, p, smem, st);
+    else if (p.rows <= 4) e = launch_decode_worker(pdec::decode_f32_kernel<D, 4>, p, smem, st);
+    else e = launch_decode_worker(pdec::decode_f32_kernel<D, 8>, p, smem, st);
   } else {
-    switch (p.rows) {
-      case 8: e = launch_decode_worker(pdec::decode_mma_kernel<T, D, 1>, p, smem, st); break;
-      case 16: e = launch_decode_worker(pdec::decode_mma_kernel<T, D, 2>, p, smem, st); break;
-      default: e = launch_decode_worker(pdec::decode_mma_kernel<T, D, 4>, p, smem, st); break;
-    }
+    if (p.rows <= 8) e = launch_decode_worker(pdec::decode_mma_kernel<T, D, 1>, p, smem, st);
+    else if (p.rows <= 16) e = launch_decode_worker(pdec::decode_mma_kernel<T, D, 2>, p, smem, st);
+    else e = launch_decode_worker(pdec::decode_mma_kernel<T, D, 4>, p, smem, st);
   }
   if (e != cudaSuccess) return e;
   // the join may start while the last workers run; it waits for them before its first read
@@ -1285,7 +1280,7 @@ int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pag
                            size_t workspace_bytes, cast_stream_t stream) {
   if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return CAST_ERR_DTYPE;
   if (B < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || num_pages < 1 || page_size < 1 || max_pages < 0 ||
-      table_stride < 0 || window < 0 || !(softcap >= 0.f))
+      table_stride < 0 || window < 0 || !(softcap == 0.f || (softcap >= 1e-6f && softcap <= 1e30f)))
     return CAST_ERR_SHAPE;
   if (D != 64 && D != 128) return CAST_ERR_HEAD_DIM;
   if (B == 0) return CAST_OK;
@@ -1317,10 +1312,15 @@ int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pag
   p.slopes = alibi_slopes;
   p.modified = softcap > 0.f || alibi_slopes != nullptr;
   p.v_minus_k = static_cast<const char*>(v_pages) - static_cast<const char*>(k_pages);
+  p.cap_exp = softcap > 0.f ? 2.f * kLog2e / softcap : 0.f;
   p.W = lay.workers;
-  // a unit has about W / units partials at most; eight of them are one warp's round in the join
+  // tails only where the table has room for groups long enough to be cut: their CTAs take 2 us to find
+  // that there is nothing for them
+  const int64_t most = (int64_t)B * (((int64_t)max_pages * page_size + pdec::KS - 1) / pdec::KS) * H_kv * p.tiles;
+  p.ns = most >= (int64_t)p.W * pdec::TAIL * pdec::MIN_TAIL ? pdec::NS : 0;
+  // a unit has about (pieces / units) partials; eight of them are one warp's round in the join
   p.join_warps = 1;
-  while (p.join_warps < 8 && (int64_t)p.join_warps * 8 * B * H_kv * p.tiles < p.W) p.join_warps *= 2;
+  while (p.join_warps < 8 && (int64_t)p.join_warps * 8 * B * H_kv * p.tiles < (int64_t)p.W * (1 + p.ns)) p.join_warps *= 2;
   p.cum = reinterpret_cast<int64_t*>(ws);
   p.ws_o = reinterpret_cast<float*>(ws + lay.o);
   p.ws_ml = reinterpret_cast<float*>(ws + lay.ml);

@@ -6,13 +6,16 @@
 // Bound: one read of the visible keys and values from HBM (4 flops per byte and query head of a KV head).
 //
 // Split: every warp is a worker of its own. The visible keys of all (sequence, KV head, tile of query
-// heads) units, in steps of KS keys, form one list of T steps; worker w of W takes steps [T w / W,
-// T (w + 1) / W), whatever units they fall into, so ragged lengths load every warp alike and no host read
-// of the lengths is needed. A worker streams its steps through a private ring of NST shared-memory stages
-// with 16-byte asynchronous copies (no block barrier in the loop; the ring runs on across units), keeps a
-// running maximum and sum, and at the end of a unit writes the output if the whole unit was its own, else
-// an unnormalised partial. The join kernel (launched to overlap the tail) adds each unit's partials in
-// worker order, so results do not depend on timing; it also writes the rows that see no key (0, -inf).
+// heads) units, in steps of KS keys, form one list of T steps, cut into n even groups of steps whatever
+// units they fall into, so ragged lengths load every warp alike and no host read of the lengths is needed.
+// A long group is cut once more, into a head and NS short tails: the CTAs of the heads come first in the
+// grid and fill the GPU, those of the tails start as slots get free. Some SMs read memory a tenth slower
+// than the others (measured: 24 of 148, always the same), and the tails go to the fast ones.
+// A worker streams its steps through a private ring of NST shared-memory stages with 16-byte asynchronous
+// copies (no block barrier in the loop; the ring runs on across units), keeps a running maximum and sum,
+// and at the end of a unit writes the output if the whole unit was its own, else an unnormalised partial.
+// The join kernel (launched to overlap the tail) adds each unit's partials in the order of the list, so
+// results do not depend on timing; it also writes the rows that see no key (0, -inf).
 //
 // 16-bit types: S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16, so that keys and head dims fill the 16
 // rows and the KV head's query heads are the 8 columns (NH tiles of them; with heads as rows a group of 4
@@ -31,6 +34,9 @@ constexpr int NW = 4;            // warps (workers) per CTA
 constexpr int NT = NW * 32;
 constexpr int KS = 16;           // keys per step
 constexpr int MIN_STEPS = 2;     // fewest steps worth a worker
+constexpr int NS = 3;            // short tails of a long group,
+constexpr int TAIL = 18;         // each 1 / TAIL of it,
+constexpr int MIN_TAIL = 4;      // and of at least this many steps
 
 // Ring stages per worker: 8 resident workers per SM hold at most 224 KB.
 template <typename T, int D> __host__ __device__ constexpr int stage_bytes() { return 2 * KS * D * (int)sizeof(T); }
@@ -50,14 +56,14 @@ struct Params {
   int B, H_q, H_kv, G, tiles, rows;                // tiles of `rows` query heads per KV head
   int num_pages, page_size, max_pages;
   int window;                                      // 0: none
-  float scale, softcap;                            // softcap 0: none
+  float scale, softcap, cap_exp;                   // softcap 0: none; 2 log2(e) / softcap
   int modified;                                    // softcap or slopes given
   int64_t v_minus_k;                               // byte distance of the value pages from the key pages
   int join_warps;                                  // warps of the join kernel per row
   const float* slopes;                             // or NULL
-  int W;                                           // workers
-  float* ws_o;                                     // [2 W][rows][D]
-  float* ws_ml;                                    // [2 W][rows][2]: running maximum (log2 units), sum
+  int W, ns;                                       // groups of steps at most; tails per group (0 or NS)
+  float* ws_o;                                     // [2 W (1 + ns)][rows][D]
+  float* ws_ml;                                    // [2 W (1 + ns)][rows][2]: running maximum (log2 units), sum
   int64_t* cum;                                    // [B + 1] first step of each sequence
 };
 
@@ -77,13 +83,28 @@ __device__ __forceinline__ Span span_of(const Params& p, int b) {
   return z;
 }
 
-// Workers that share T steps, and worker w's first step.
-__device__ __forceinline__ int active_workers(int64_t T, int W) {
-  const int64_t n = (T + MIN_STEPS - 1) / MIN_STEPS;
-  return n < W ? (int)n : W;
-}
-__device__ __forceinline__ int64_t first_step(int64_t T, int n, int w) { return T * w / n; }
-__device__ __forceinline__ int worker_of(int64_t T, int n, int64_t step) { return (int)(((step + 1) * n + T - 1) / T) - 1; }
+// How T steps are cut: n groups, group g = steps [T g / n, T (g + 1) / n), of which the last ns * tail are
+// ns tails. Piece j of group g (0: its head) is piece g (1 + ns) + j of the list.
+struct Cut {
+  int64_t T;
+  int n, ns, tail;
+  __device__ __forceinline__ Cut(int64_t steps, int W, int tails) : T(steps) {
+    const int64_t m = (T + MIN_STEPS - 1) / MIN_STEPS;
+    n = m < W ? (int)m : W;
+    tail = tails > 0 && n > 0 ? (int)(T / n / TAIL) : 0;
+    ns = tail >= MIN_TAIL ? tails : 0;
+  }
+  __device__ __forceinline__ int64_t group(int g) const { return T * g / n; }
+  __device__ __forceinline__ int64_t first(int g, int j) const {
+    return j == 0 ? group(g) : group(g + 1) - (int64_t)(ns - j + 1) * tail;
+  }
+  __device__ __forceinline__ int piece_of(int64_t step) const {
+    const int g = (int)(((step + 1) * n + T - 1) / T) - 1;
+    if (ns == 0) return g;
+    const int64_t back = group(g + 1) - 1 - step;
+    return g * (1 + ns) + (back < (int64_t)ns * tail ? ns - (int)(back / tail) : 0);
+  }
+};
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -143,9 +164,21 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A scaled score with its cap and its bias by the distance to the newest key, in log2 units.
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A scaled score with its cap and its bias by the distance to the newest key, in log2 units. 16-bit types
+// take tanh x = 1 - 2 / (1 + e^2x), off by some 2^-22 of the cap (tanhf took a third of the loop's
+// instructions); 32-bit keeps tanhf.
+template <bool EXACT>
 __device__ __forceinline__ float modified_score(const Params& p, float s, int n, const Span& z, float slope) {
-  if (p.softcap > 0.f) s = p.softcap * tanhf(s / p.softcap);
+  if (p.softcap > 0.f) {
+    if (EXACT) s = p.softcap * tanhf(s / p.softcap);
+    else s = fmaf(-2.f * p.softcap, rcp(1.f + ex2(s * p.cap_exp)), p.softcap);
+  }
   if (p.slopes != nullptr) s = fmaf(slope, (float)(n - (z.len - 1)), s);
   return s * kLog2e;
 }
@@ -174,13 +207,15 @@ __device__ __forceinline__ bool advance(const Params& p, Cursor& c) {
   return true;
 }
 
-// First step of every sequence: the block sums its threads' runs of sequences, scans the sums and finds
-// the sequence that holds worker w's first step. CTA 0 writes the list for the join kernel.
-struct Plan {
-  int64_t T;
-  int n;            // workers that take part
+// What this warp does: its piece of the list and the cursor at the piece's first step.
+struct Work {
+  int piece;        // -1: nothing
+  int steps;
+  Cursor c;
 };
-__device__ __forceinline__ Plan plan_steps(const Params& p, int w, Cursor& c, int64_t& begin, int64_t& end) {
+// The block sums its threads' runs of sequences, scans the sums and finds the sequence that holds the
+// piece's first step. CTA 0 writes each sequence's first step for the join kernel.
+__device__ __forceinline__ Work plan_steps(const Params& p) {
   __shared__ int64_t sums[NT + 1];
   const int tid = threadIdx.x, lane = tid & 31;
   const int per = (p.B + NT - 1) / NT;
@@ -215,12 +250,22 @@ __device__ __forceinline__ Plan plan_steps(const Params& p, int w, Cursor& c, in
     }
     if (tid == 0) p.cum[p.B] = sums[NT];
   }
-  Plan pl;
-  pl.T = sums[NT];
-  pl.n = active_workers(pl.T, p.W);
-  if (w >= pl.n) return pl;
-  begin = first_step(pl.T, pl.n, w);
-  end = first_step(pl.T, pl.n, w + 1);
+  const Cut cut(sums[NT], p.W, p.ns);
+  Work wk;
+  Cursor& c = wk.c;
+  wk.piece = -1;
+  // the heads' CTAs come first; tail CTA x takes tail x % NS of four neighbouring groups
+  const int heads = p.W / NW;
+  int g = blockIdx.x * NW + (tid >> 5), j = 0;
+  if ((int)blockIdx.x >= heads) {
+    const int x = blockIdx.x - heads;
+    g = x / NS * NW + (tid >> 5);
+    j = 1 + x % NS;
+  }
+  if (g >= cut.n || j > cut.ns) return wk;
+  wk.piece = g * (1 + cut.ns) + j;
+  const int64_t begin = cut.first(g, j);
+  wk.steps = (int)((j == cut.ns ? cut.group(g + 1) : cut.first(g, j + 1)) - begin);
   // the run of sequences that holds step `begin`: the last thread whose first step is <= begin
   int cnt = 0;
   for (int i = 0; i < NT / 32; ++i) cnt += __popc(__ballot_sync(0xffffffffu, sums[i * 32 + lane] <= begin));
@@ -237,67 +282,71 @@ __device__ __forceinline__ Plan plan_steps(const Params& p, int w, Cursor& c, in
   const int steps = c.z.s1 - c.z.s0;
   c.u = (int)((begin - at) / steps);
   c.s = c.z.s0 + (int)((begin - at) % steps);
-  return pl;
+  return wk;
 }
 
-// The copying side of a worker: its own cursor, ahead of the computing one, and the page of its step,
-// read from the table while the step before it is being copied.
+// The copying side of a worker: its own cursor, ahead of the computing one. Where page_size is a multiple
+// of KS a step lies in one page: lane i holds the table entry of the i-th step from `base`, and those of
+// the 32 steps after are under way. Else every lane reads the entry of its key, a step ahead.
 // A stage holds KS rows of keys, then of values; 16-byte piece c of row r is kept at c ^ (r & 7), so that
 // row-wise and piece-wise reads meet all banks.
 template <typename T, int D>
 struct Copier {
   static constexpr int CH = D * (int)sizeof(T) / 16;      // pieces per row
-  static constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;   // rows per warp-wide copy
+  static constexpr int RPI = 32 / CH;                     // rows per warp-wide copy
   static constexpr int IT = KS * CH / 32;                 // copies per step (keys or values)
   static constexpr int ROW = D * (int)sizeof(T);
   Cursor c;
-  int page;               // page_size % KS == 0: the step's page; else the page of key lane & 15
-  int pi, pr;             // page_size % KS == 0: page index and first row of the step
+  int page, ahead;        // see above
+  int base, pr;           // page_size % KS == 0: first step of `page`, row of its page where step c.s starts
   const char* head;       // keys of the unit's KV head
 
+  __device__ __forceinline__ int entry(const Params& p, int step) const {
+    return step < c.z.s1 ? p.table[(int64_t)c.b * p.table_stride + step * KS / p.page_size] : -1;
+  }
+  __device__ __forceinline__ int key_entry(const Params& p) const {
+    const int n = c.s * KS + (threadIdx.x & 15);
+    return (n >= c.z.lo && n < c.z.len) ? p.table[(int64_t)c.b * p.table_stride + n / p.page_size] : -1;
+  }
   __device__ __forceinline__ void enter(const Params& p) {
     head = static_cast<const char*>(p.k) + (int64_t)(c.u / p.tiles) * p.s_h * (int)sizeof(T);
     if (p.page_size % KS == 0) {
-      const int n0 = c.s * KS;
-      pi = n0 / p.page_size;
-      pr = n0 - pi * p.page_size;
-    }
-  }
-  __device__ __forceinline__ void fetch(const Params& p) {
-    const int32_t* row = p.table + (int64_t)c.b * p.table_stride;
-    if (p.page_size % KS == 0) {
-      page = row[pi];
+      base = c.s;
+      pr = c.s * KS % p.page_size;
+      page = entry(p, base + (threadIdx.x & 31));
+      ahead = entry(p, base + 32 + (threadIdx.x & 31));
     } else {
-      const int n = c.s * KS + (threadIdx.x & 15);
-      page = (n >= c.z.lo && n < c.z.len) ? row[n / p.page_size] : -1;
+      page = key_entry(p);
     }
   }
   __device__ __forceinline__ void start(const Params& p, const Cursor& at) {
     c = at;
     enter(p);
-    fetch(p);
   }
   __device__ __forceinline__ void next(const Params& p) {
     if (advance(p, c)) {
       enter(p);
     } else if (p.page_size % KS == 0) {
-      pr += KS;
-      if (pr == p.page_size) {
-        pr = 0;
-        ++pi;
+      pr = pr + KS == p.page_size ? 0 : pr + KS;
+      if (c.s == base + 32) {
+        base = c.s;
+        page = ahead;
+        ahead = entry(p, base + 32 + (threadIdx.x & 31));
       }
+    } else {
+      page = key_entry(p);
     }
-    fetch(p);
   }
   __device__ __forceinline__ void copy(const Params& p, uint32_t stage) const {
     const int lane = threadIdx.x & 31;
     const int ch = lane % CH, r0 = lane / CH;
     const int lo = c.z.lo - c.s * KS, hi = c.z.len - c.s * KS;     // visible rows of the step: [lo, hi)
     if (p.page_size % KS == 0) {
-      const bool ok = page >= 0 && page < p.num_pages;
+      const int pg = __shfl_sync(0xffffffffu, page, c.s - base);
+      const bool ok = pg >= 0 && pg < p.num_pages;
       if (!ok) report(CAST_DEV_BAD_LAYOUT);
       const int64_t step = p.s_r * (int)sizeof(T) * RPI;
-      const char* src = head + ((int64_t)(ok ? page : 0) * p.s_p + (int64_t)(pr + r0) * p.s_r) * (int)sizeof(T) + ch * 16;
+      const char* src = head + ((int64_t)(ok ? pg : 0) * p.s_p + (int64_t)(pr + r0) * p.s_r) * (int)sizeof(T) + ch * 16;
       if (ok && lo <= 0 && hi >= KS) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
@@ -350,13 +399,11 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
   constexpr int NST = stages<T, D>(), SB = stage_bytes<T, D>(), ROW = D * 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int w = blockIdx.x * NW + warp;
-  Cursor cc;
-  int64_t begin = 0, end = 0;
-  const Plan pl = plan_steps(p, w, cc, begin, end);
-  if (w >= pl.n) return;
+  const Work wk = plan_steps(p);
+  if (wk.piece < 0) return;
+  Cursor cc = wk.c;
   const uint32_t ring = tc::smem_u32(smem) + warp * NST * SB;
-  int left = (int)(end - begin);       // steps to compute
+  int left = wk.steps;                 // steps to compute
   int to_copy = left;
   Copier<T, D> cp;
   cp.start(p, cc);
@@ -382,7 +429,7 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
   float o[NH][D / 16][4], m[NH][2], l[NH][2], slope[NH][2];
   bool fresh = true;                   // the next step starts a piece of a unit
   bool whole = false;                  // that piece starts at the unit's first step
-  int slot = 2 * w;
+  int slot = 2 * wk.piece;
   int h0 = 0, nrow = 0;
   for (; left > 0; --left) {
     if (fresh) {
@@ -419,25 +466,31 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
     take = take + SB == ring + NST * SB ? ring : take + SB;
     issue();                           // into the stage that the previous step left
 
-    float s[NH][4];
+    constexpr int NC = NH == 1 ? 2 : 1;      // one tile of heads: two chains of dependent MMAs
+    float s[NH][4], s2[NH][4];
 #pragma unroll
     for (int a = 0; a < NH; ++a)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[a][i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[a][i] = s2[a][i] = 0.f;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       uint32_t ka[4];
       ldsm4(st + koff + ((kx ^ (2 * k)) * 16), ka);
 #pragma unroll
-      for (int a = 0; a < NH; ++a) mma16816<T>(s[a], ka, qf[a][k][0], qf[a][k][1]);
+      for (int a = 0; a < NH; ++a) mma16816<T>((k % NC) ? s2[a] : s[a], ka, qf[a][k][0], qf[a][k][1]);
     }
+    if (NC == 2)
+#pragma unroll
+      for (int a = 0; a < NH; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[a][i] += s2[a][i];
     const int n0 = cc.s * KS + g;
     if (p.modified) {
 #pragma unroll
       for (int a = 0; a < NH; ++a)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          s[a][i] = modified_score(p, s[a][i] * p.scale, n0 + (i >> 1) * 8, cc.z, slope[a][i & 1]);
+          s[a][i] = modified_score<false>(p, s[a][i] * p.scale, n0 + (i >> 1) * 8, cc.z, slope[a][i & 1]);
     } else {
 #pragma unroll
       for (int a = 0; a < NH; ++a)
@@ -526,7 +579,7 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
             if (g == 0) *reinterpret_cast<float2*>(p.ws_ml + ((int64_t)slot * p.rows + r) * 2) = make_float2(m[a][i], lt);
           }
         }
-      slot = 2 * w + 1;
+      slot = 2 * wk.piece + 1;
       fresh = true;
     }
     if (left > 1) advance(p, cc);
@@ -546,14 +599,12 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
   __shared__ __align__(16) float sq[NW][GT][D];
   __shared__ __align__(16) float sp[NW][GT][KS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int w = blockIdx.x * NW + warp;
-  Cursor cc;
-  int64_t begin = 0, end = 0;
-  const Plan pl = plan_steps(p, w, cc, begin, end);
-  if (w >= pl.n) return;
+  const Work wk = plan_steps(p);
+  if (wk.piece < 0) return;
+  Cursor cc = wk.c;
   uint8_t* ring_p = smem + (size_t)warp * NST * SB;
   const uint32_t ring = tc::smem_u32(ring_p);
-  int left = (int)(end - begin), to_copy = left;
+  int left = wk.steps, to_copy = left;
   Copier<float, D> cp;
   cp.start(p, cc);
   uint32_t put = 0, take = 0;
@@ -569,7 +620,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
 
   float o[GT][DV], m[GT], l[GT], slope[GT];
   bool fresh = true, whole = false;
-  int slot = 2 * w, h0 = 0, nrow = 0;
+  int slot = 2 * wk.piece, h0 = 0, nrow = 0;
   const int key = lane & 15, half = lane >> 4;
   const float c = p.scale * kLog2e;
   for (; left > 0; --left) {
@@ -617,7 +668,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
 #pragma unroll
     for (int a = 0; a < GT; ++a) {
       s[a] += __shfl_xor_sync(0xffffffffu, s[a], 16);
-      s[a] = p.modified ? modified_score(p, s[a] * p.scale, n, cc.z, slope[a]) : s[a] * c;
+      s[a] = p.modified ? modified_score<true>(p, s[a] * p.scale, n, cc.z, slope[a]) : s[a] * c;
       if (n < cc.z.lo || n >= cc.z.len) s[a] = -INFINITY;
       float mx = s[a];
 #pragma unroll
@@ -680,7 +731,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
 #pragma unroll
         for (int i = 0; i < DV; ++i) dst[lane * DV + i] = o[a][i] * f;
       }
-      slot = 2 * w + 1;
+      slot = 2 * wk.piece + 1;
       fresh = true;
     }
     __syncwarp();
@@ -692,7 +743,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
 // ---------------------------------------------------------------------------------------- join
 // Adds the partials of each (sequence, query head), in worker order: join_warps warps take every
 // join_warps-th one of a row's partials, eight at a time (their sums and outputs are loaded together),
-// and the first adds up the warps' results. Units that one worker took whole are already written; rows
+// and the first adds up the warps' results. Units that one piece held whole are already written; rows
 // without a visible key become 0 (lse -inf).
 template <typename T, int D>
 __global__ void __launch_bounds__(JOIN_NT) decode_join_kernel(const Params p) {
@@ -709,17 +760,17 @@ __global__ void __launch_bounds__(JOIN_NT) decode_join_kernel(const Params p) {
   const int64_t c0 = p.cum[b], c1 = p.cum[b + 1];
   const int units = p.H_kv * p.tiles;
   T* out = static_cast<T*>(p.out) + (int64_t)b * p.so_b + (int64_t)hq * p.so_h;
-  int w0 = 0, w1 = 0, first = 0, r = 0;
+  int w0 = 0, w1 = 0, first = 0, r = 0;      // pieces of the row's unit
   const bool split = have && c1 != c0;
   if (split) {
     const int64_t steps = (c1 - c0) / units;
     const int hr = hq % p.G, u = (hq / p.G) * p.tiles + hr / p.rows;
     r = hr % p.rows;
     const int64_t us = c0 + u * steps;
-    const int n = active_workers(T_all, p.W);
-    w0 = worker_of(T_all, n, us);
-    w1 = worker_of(T_all, n, us + steps - 1);
-    first = 2 * w0 + (first_step(T_all, n, w0) == us ? 0 : 1);
+    const Cut cut(T_all, p.W, p.ns);
+    w0 = cut.piece_of(us);
+    w1 = cut.piece_of(us + steps - 1);
+    first = 2 * w0 + (cut.first(w0 / (1 + cut.ns), w0 % (1 + cut.ns)) == us ? 0 : 1);
   }
   float M = -INFINITY, L = 0.f, acc[DV];
 #pragma unroll

@@ -205,8 +205,8 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     if rows != B:
         raise ValueError("decode_attention_paged: page_table must have one row per sequence")
     seq_len = _i32(seq_len, dev, "seq_len", B)
-    if window < 0 or not softcap >= 0.0:
-        raise ValueError("decode_attention_paged: window and softcap must not be negative")
+    if window < 0 or not (softcap == 0.0 or 1e-6 <= softcap <= 1e30):
+        raise ValueError("decode_attention_paged: window must not be negative, softcap 0 or 1e-6 to 1e30")
     q = _prep(q)
     if out is None:
         out = torch.empty_like(q)

@@ -438,7 +438,7 @@ int cast_paged_append(int n_layers, void* const* pages_kv, const void* const* ne
  * Attention of one new token per sequence over its pages. q / out: [B, H_q, D];
  * seq_len [B] counts the keys, the new token's own among them. Scores are
  * q . k * sm_scale (<= 0: 1/sqrt(D)), then, where given, softcap * tanh(s / softcap)
- * (softcap > 0), then + alibi_slopes[head] * (n - (seq_len - 1)) (float [H_q]); keys
+ * (0: none; else 1e-6 to 1e30), then + alibi_slopes[head] * (n - (seq_len - 1)) (float [H_q]); keys
  * n < seq_len - window are not seen (window > 0). lse (float [B, H_q], or NULL)
  * receives the natural log of the sum of the exponentials. A sequence without keys
  * gives 0 and -inf. strides[7] = q (batch, head), pages (page, head, row; keys and

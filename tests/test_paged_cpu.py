@@ -57,7 +57,7 @@ def _decode(L, **o):
 def test_decode_argument_checks(L):
     assert _decode(L, dtype=3) == -3
     assert _decode(L, Hq=30) == -2 and _decode(L, np=0) == -2 and _decode(L, ps=0) == -2 and _decode(L, win=-1) == -2
-    assert _decode(L, cap=-1.0) == -2 and _decode(L, cap=float("nan")) == -2
+    assert all(_decode(L, cap=x) == -2 for x in (-1.0, 1e-7, 1e31, float("inf"), float("nan")))
     assert _decode(L, D=96) == -4
     assert _decode(L, q=None) == -1 and _decode(L, table=None) == -1 and _decode(L, sl=None) == -1
     assert _decode(L, q=P + 8) == -7 and _decode(L, k=P + 8) == -7
