@@ -1136,12 +1136,6 @@ int decode_rows(int dtype, int G) {
   return std::min(G, dtype == CAST_F32 ? 8 : 32);
 }
 
-int decode_workers(int dtype, int D, int sms) {
-  const int per_sm = dtype == CAST_F32 ? (D == 128 ? pdec::ctas_per_sm<float, 128>() : pdec::ctas_per_sm<float, 64>())
-                                       : (D == 128 ? pdec::ctas_per_sm<__half, 128>() : pdec::ctas_per_sm<__half, 64>());
-  return sms * per_sm * pdec::NW;
-}
-
 // Workspace: first steps [B + 1] int64, then the partials of two units per piece of the step list.
 struct DecodeLayout {
   int rows, workers;
@@ -1150,7 +1144,7 @@ struct DecodeLayout {
 DecodeLayout decode_layout(int dtype, int B, int G, int D, int sms) {
   DecodeLayout l;
   l.rows = decode_rows(dtype, G);
-  l.workers = decode_workers(dtype, D, sms);
+  l.workers = sms * pdec::CTAS_PER_SM * pdec::NW;
   const size_t slots = 2 * (size_t)l.workers * (1 + pdec::NS) * l.rows;
   l.o = align256((size_t)(B + 1) * sizeof(int64_t));
   l.ml = l.o + align256(slots * D * sizeof(float));
@@ -1316,7 +1310,10 @@ int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pag
   p.W = lay.workers;
   // tails only where the table has room for groups long enough to be cut: their CTAs take 2 us to find
   // that there is nothing for them
-  const int64_t most = (int64_t)B * (((int64_t)max_pages * page_size + pdec::KS - 1) / pdec::KS) * H_kv * p.tiles;
+  const int ks = dtype == CAST_F32 && D == 128 ? pdec::step_keys<float, 128>() : pdec::step_keys<__half, 128>();
+  int64_t keys = (int64_t)max_pages * page_size;
+  if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + ks);
+  const int64_t most = (int64_t)B * ((keys + ks - 1) / ks) * H_kv * p.tiles;
   p.ns = most >= (int64_t)p.W * pdec::TAIL * pdec::MIN_TAIL ? pdec::NS : 0;
   // a unit has about (pieces / units) partials; eight of them are one warp's round in the join
   p.join_warps = 1;

@@ -6,7 +6,7 @@
 // Bound: one read of the visible keys and values from HBM (4 flops per byte and query head of a KV head).
 //
 // Split: every warp is a worker of its own. The visible keys of all (sequence, KV head, tile of query
-// heads) units, in steps of KS keys, form one list of T steps, cut into n even groups of steps whatever
+// heads) units, in steps of 16 keys (8 in 32 bits at D = 128), form one list of T steps, cut into n even groups of steps whatever
 // units they fall into, so ragged lengths load every warp alike and no host read of the lengths is needed.
 // A long group is cut once more, into a head and NS short tails: the CTAs of the heads come first in the
 // grid and fill the GPU, those of the tails start as slots get free. Some SMs read memory a tenth slower
@@ -32,18 +32,15 @@ namespace pdec {
 
 constexpr int NW = 4;            // warps (workers) per CTA
 constexpr int NT = NW * 32;
-constexpr int KS = 16;           // keys per step
-constexpr int MIN_STEPS = 2;     // fewest steps worth a worker
-constexpr int NS = 3;            // short tails of a long group,
-constexpr int TAIL = 18;         // each 1 / TAIL of it,
-constexpr int MIN_TAIL = 4;      // and of at least this many steps
+constexpr int NS = 2;            // short tails of a long group,
+constexpr int TAIL = 12;         // each 1 / TAIL of it,
+constexpr int MIN_TAIL = 8;      // and of at least this many steps (tails of 4 cost a sequence of 131072 keys a tenth)
 
-// Ring stages per worker: 8 resident workers per SM hold at most 224 KB.
-template <typename T, int D> __host__ __device__ constexpr int stage_bytes() { return 2 * KS * D * (int)sizeof(T); }
-template <typename T, int D> __host__ __device__ constexpr int stages() {
-  return sizeof(T) == 4 ? (D == 128 ? 3 : 6) : (D == 128 ? 3 : 6);
-}
-template <typename T, int D> __host__ __device__ constexpr int ctas_per_sm() { return sizeof(T) == 4 ? 1 : 2; }
+// Keys per step, and ring stages per worker: eight workers per SM (two CTAs) hold 192 KB.
+template <typename T, int D> __host__ __device__ constexpr int step_keys() { return sizeof(T) == 4 && D == 128 ? 8 : 16; }
+template <typename T, int D> __host__ __device__ constexpr int stage_bytes() { return 2 * step_keys<T, D>() * D * (int)sizeof(T); }
+template <typename T, int D> __host__ __device__ constexpr int stages() { return 24 * 1024 / stage_bytes<T, D>(); }
+constexpr int CTAS_PER_SM = 2;
 constexpr int JOIN_NT = 256;
 
 struct Params {
@@ -71,7 +68,7 @@ struct Params {
 struct Span {
   int lo, len, s0, s1;
 };
-__device__ __forceinline__ Span span_of(const Params& p, int b) {
+template <int KS> __device__ __forceinline__ Span span_of(const Params& p, int b) {
   Span z;
   int len = p.seq_len[b];
   // out of range (reported by plan_steps): nothing is visible
@@ -89,8 +86,7 @@ struct Cut {
   int64_t T;
   int n, ns, tail;
   __device__ __forceinline__ Cut(int64_t steps, int W, int tails) : T(steps) {
-    const int64_t m = (T + MIN_STEPS - 1) / MIN_STEPS;
-    n = m < W ? (int)m : W;
+    n = T < W ? (int)T : W;
     tail = tails > 0 && n > 0 ? (int)(T / n / TAIL) : 0;
     ns = tail >= MIN_TAIL ? tails : 0;
   }
@@ -194,13 +190,14 @@ struct Cursor {
   Span z;
 };
 // To the next step; true when it starts another unit.
+template <int KS>
 __device__ __forceinline__ bool advance(const Params& p, Cursor& c) {
   if (++c.s < c.z.s1) return false;
   if (++c.u == p.H_kv * p.tiles) {
     c.u = 0;
     do {
       if (++c.b >= p.B) return true;
-      c.z = span_of(p, c.b);
+      c.z = span_of<KS>(p, c.b);
     } while (c.z.s1 <= c.z.s0);
   }
   c.s = c.z.s0;
@@ -215,6 +212,7 @@ struct Work {
 };
 // The block sums its threads' runs of sequences, scans the sums and finds the sequence that holds the
 // piece's first step. CTA 0 writes each sequence's first step for the join kernel.
+template <int KS>
 __device__ __forceinline__ Work plan_steps(const Params& p) {
   __shared__ int64_t sums[NT + 1];
   const int tid = threadIdx.x, lane = tid & 31;
@@ -223,7 +221,7 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
   const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) {
-    const Span z = span_of(p, b);
+    const Span z = span_of<KS>(p, b);
     mine += (z.s1 - z.s0) * units;
     if (blockIdx.x == 0 && z.len != p.seq_len[b]) report(CAST_DEV_BAD_LAYOUT);
   }
@@ -245,7 +243,7 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
     int64_t at = sums[tid];
     for (int b = b0; b < b1; ++b) {
       p.cum[b] = at;
-      const Span z = span_of(p, b);
+      const Span z = span_of<KS>(p, b);
       at += (z.s1 - z.s0) * units;
     }
     if (tid == 0) p.cum[p.B] = sums[NT];
@@ -272,7 +270,7 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
   int b = (cnt - 1) * per;
   int64_t at = sums[cnt - 1];
   while (true) {
-    c.z = span_of(p, b);
+    c.z = span_of<KS>(p, b);
     const int64_t n = (c.z.s1 - c.z.s0) * units;
     if (begin < at + n) break;
     at += n;
@@ -285,64 +283,57 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
   return wk;
 }
 
-// The copying side of a worker: its own cursor, ahead of the computing one. Where page_size is a multiple
-// of KS a step lies in one page: lane i holds the table entry of the i-th step from `base`, and those of
-// the 32 steps after are under way. Else every lane reads the entry of its key, a step ahead.
+// The copying side of a worker: its own cursor, ahead of the computing one. Lane i holds the sequence's
+// table entry `base` + i, and entry `base` + 32 + i is under way.
 // A stage holds KS rows of keys, then of values; 16-byte piece c of row r is kept at c ^ (r & 7), so that
 // row-wise and piece-wise reads meet all banks.
 template <typename T, int D>
 struct Copier {
+  static constexpr int KS = step_keys<T, D>();
   static constexpr int CH = D * (int)sizeof(T) / 16;      // pieces per row
   static constexpr int RPI = 32 / CH;                     // rows per warp-wide copy
   static constexpr int IT = KS * CH / 32;                 // copies per step (keys or values)
   static constexpr int ROW = D * (int)sizeof(T);
   Cursor c;
-  int page, ahead;        // see above
-  int base, pr;           // page_size % KS == 0: first step of `page`, row of its page where step c.s starts
+  int base, page, ahead;
+  int pi, pr;             // page and row of the step's first key
   const char* head;       // keys of the unit's KV head
 
-  __device__ __forceinline__ int entry(const Params& p, int step) const {
-    return step < c.z.s1 ? p.table[(int64_t)c.b * p.table_stride + step * KS / p.page_size] : -1;
-  }
-  __device__ __forceinline__ int key_entry(const Params& p) const {
-    const int n = c.s * KS + (threadIdx.x & 15);
-    return (n >= c.z.lo && n < c.z.len) ? p.table[(int64_t)c.b * p.table_stride + n / p.page_size] : -1;
-  }
-  __device__ __forceinline__ void enter(const Params& p) {
-    head = static_cast<const char*>(p.k) + (int64_t)(c.u / p.tiles) * p.s_h * (int)sizeof(T);
-    if (p.page_size % KS == 0) {
-      base = c.s;
-      pr = c.s * KS % p.page_size;
-      page = entry(p, base + (threadIdx.x & 31));
-      ahead = entry(p, base + 32 + (threadIdx.x & 31));
-    } else {
-      page = key_entry(p);
-    }
+  __device__ __forceinline__ int entry(const Params& p, int i) const {
+    return i <= (c.z.len - 1) / p.page_size ? p.table[(int64_t)c.b * p.table_stride + i] : -1;
   }
   __device__ __forceinline__ void start(const Params& p, const Cursor& at) {
+    const int lane = threadIdx.x & 31, n0 = at.s * KS;
     c = at;
-    enter(p);
+    head = static_cast<const char*>(p.k) + (int64_t)(c.u / p.tiles) * p.s_h * (int)sizeof(T);
+    pi = n0 / p.page_size;
+    pr = n0 - pi * p.page_size;
+    base = pi;
+    page = entry(p, base + lane);
+    ahead = entry(p, base + 32 + lane);
   }
   __device__ __forceinline__ void next(const Params& p) {
-    if (advance(p, c)) {
-      enter(p);
-    } else if (p.page_size % KS == 0) {
-      pr = pr + KS == p.page_size ? 0 : pr + KS;
-      if (c.s == base + 32) {
-        base = c.s;
-        page = ahead;
-        ahead = entry(p, base + 32 + (threadIdx.x & 31));
-      }
-    } else {
-      page = key_entry(p);
+    if (advance<KS>(p, c)) {
+      start(p, c);
+      return;
+    }
+    pr += KS;
+    while (pr >= p.page_size) {
+      pr -= p.page_size;
+      ++pi;
+    }
+    if (pi >= base + 32) {      // by 16 at most
+      base += 32;
+      page = ahead;
+      ahead = entry(p, base + 32 + (threadIdx.x & 31));
     }
   }
   __device__ __forceinline__ void copy(const Params& p, uint32_t stage) const {
     const int lane = threadIdx.x & 31;
     const int ch = lane % CH, r0 = lane / CH;
     const int lo = c.z.lo - c.s * KS, hi = c.z.len - c.s * KS;     // visible rows of the step: [lo, hi)
-    if (p.page_size % KS == 0) {
-      const int pg = __shfl_sync(0xffffffffu, page, c.s - base);
+    if (pr + KS <= p.page_size) {          // one page (always where page_size is a multiple of KS)
+      const int pg = __shfl_sync(0xffffffffu, page, pi - base);
       const bool ok = pg >= 0 && pg < p.num_pages;
       if (!ok) report(CAST_DEV_BAD_LAYOUT);
       const int64_t step = p.s_r * (int)sizeof(T) * RPI;
@@ -368,17 +359,18 @@ struct Copier {
         }
       }
     } else {
-      const int n = c.s * KS + (lane & 15);
+      const int key = lane & (KS - 1), i = (pr + key) / p.page_size, row = pr + key - i * p.page_size;
+      const int e = pi + i - base;         // up to 31 + KS
+      const int e0 = __shfl_sync(0xffffffffu, page, e & 31), e1 = __shfl_sync(0xffffffffu, ahead, e & 31);
+      const int pg = e < 32 ? e0 : e1;
       int64_t off = -1;
-      if (n >= c.z.lo && n < c.z.len) {
-        if (page >= 0 && page < p.num_pages)
-          off = ((int64_t)page * p.s_p + (int64_t)(n % p.page_size) * p.s_r) * (int)sizeof(T);
-        else
-          report(CAST_DEV_BAD_LAYOUT);
+      if (key >= lo && key < hi) {
+        if (pg >= 0 && pg < p.num_pages) off = ((int64_t)pg * p.s_p + (int64_t)row * p.s_r) * (int)sizeof(T);
+        else report(CAST_DEV_BAD_LAYOUT);
       }
 #pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const int r = i * RPI + r0;
+      for (int k = 0; k < IT; ++k) {
+        const int r = k * RPI + r0;
         const int64_t o = __shfl_sync(0xffffffffu, off, r);
         const char* src = head + (o >= 0 ? o : 0) + ch * 16;
         const uint32_t dst = stage + r * ROW + ((ch ^ (r & 7)) * 16);
@@ -396,10 +388,10 @@ template <typename T, int D, int NH>
 __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int NST = stages<T, D>(), SB = stage_bytes<T, D>(), ROW = D * 2;
+  constexpr int KS = step_keys<T, D>(), NST = stages<T, D>(), SB = stage_bytes<T, D>(), ROW = D * 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  const Work wk = plan_steps(p);
+  const Work wk = plan_steps<KS>(p);
   if (wk.piece < 0) return;
   Cursor cc = wk.c;
   const uint32_t ring = tc::smem_u32(smem) + warp * NST * SB;
@@ -582,24 +574,24 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
       slot = 2 * wk.piece + 1;
       fresh = true;
     }
-    if (left > 1) advance(p, cc);
+    if (left > 1) advance<KS>(p, cc);
   }
   cp_wait<0>();
 }
 
 // ---------------------------------------------------------------------------------------- 32-bit type
-// GT query heads of one KV head. Scores: lane = key (lane & 15) and half of the head dim (lane >> 4);
-// outputs: lane = D / 32 dims, over the step's 16 keys.
+// GT query heads of one KV head. Scores: lane = key (lane % KS) and part of the head dim (lane / KS);
+// outputs: lane = D / 32 dims, over the step's keys.
 template <int D, int GT>
 __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int NST = stages<float, D>(), SB = stage_bytes<float, D>();
-  constexpr int DV = D / 32;
+  constexpr int KS = step_keys<float, D>(), NST = stages<float, D>(), SB = stage_bytes<float, D>();
+  constexpr int DV = D / 32, PARTS = 32 / KS;
   __shared__ __align__(16) float sq[NW][GT][D];
   __shared__ __align__(16) float sp[NW][GT][KS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const Work wk = plan_steps(p);
+  const Work wk = plan_steps<KS>(p);
   if (wk.piece < 0) return;
   Cursor cc = wk.c;
   uint8_t* ring_p = smem + (size_t)warp * NST * SB;
@@ -621,7 +613,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
   float o[GT][DV], m[GT], l[GT], slope[GT];
   bool fresh = true, whole = false;
   int slot = 2 * wk.piece, h0 = 0, nrow = 0;
-  const int key = lane & 15, half = lane >> 4;
+  const int key = lane % KS, part = lane / KS;
   const float c = p.scale * kLog2e;
   for (; left > 0; --left) {
     if (fresh) {
@@ -652,8 +644,8 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
 #pragma unroll
     for (int a = 0; a < GT; ++a) s[a] = 0.f;
 #pragma unroll 4
-    for (int i = 0; i < D / 8; ++i) {
-      const int ch = half * (D / 8) + i;
+    for (int i = 0; i < D / 4 / PARTS; ++i) {
+      const int ch = part * (D / 4 / PARTS) + i;
       const float4 x = *reinterpret_cast<const float4*>(st + key * (D * 4) + ((ch ^ (key & 7)) * 16));
 #pragma unroll
       for (int a = 0; a < GT; ++a) {
@@ -667,12 +659,13 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
     const int n = cc.s * KS + key;
 #pragma unroll
     for (int a = 0; a < GT; ++a) {
-      s[a] += __shfl_xor_sync(0xffffffffu, s[a], 16);
+#pragma unroll
+      for (int i = KS; i < 32; i <<= 1) s[a] += __shfl_xor_sync(0xffffffffu, s[a], i);
       s[a] = p.modified ? modified_score<true>(p, s[a] * p.scale, n, cc.z, slope[a]) : s[a] * c;
       if (n < cc.z.lo || n >= cc.z.len) s[a] = -INFINITY;
       float mx = s[a];
 #pragma unroll
-      for (int i = 1; i < 16; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
+      for (int i = 1; i < KS; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
       const float mn = fmaxf(m[a], mx);
       const float al = mn == -INFINITY ? 1.f : exp2f(m[a] - mn);
       const float pv = mn == -INFINITY ? 0.f : exp2f(s[a] - mn);
@@ -680,7 +673,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
       l[a] = l[a] * al + pv;            // this lane's key; joined at the end of the unit
 #pragma unroll
       for (int i = 0; i < DV; ++i) o[a][i] *= al;
-      if (half == 0) sp[warp][a][key] = pv;
+      if (part == 0) sp[warp][a][key] = pv;
     }
     __syncwarp();
     const uint8_t* vt = st + KS * D * 4;
@@ -715,7 +708,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
       for (int a = 0; a < GT; ++a) {
         float lt = l[a];
 #pragma unroll
-        for (int i = 1; i < 16; i <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, i);
+        for (int i = 1; i < KS; i <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, i);
         if (a >= nrow) continue;
         float* dst;
         float f = 1.f;
@@ -735,7 +728,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
       fresh = true;
     }
     __syncwarp();
-    if (left > 1) advance(p, cc);
+    if (left > 1) advance<KS>(p, cc);
   }
   cp_wait<0>();
 }
