@@ -1154,7 +1154,8 @@ DecodeLayout decode_layout(int dtype, int B, int G, int D, int sms) {
 
 template <typename K>
 cudaError_t launch_decode_worker(K kern, const pdec::Params& p, size_t smem, cudaStream_t st) {
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
   kern<<<p.W / pdec::NW * (1 + p.ns), pdec::NT, smem, st>>>(p);
   return cudaGetLastError();
 }

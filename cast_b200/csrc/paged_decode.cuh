@@ -68,9 +68,8 @@ struct Params {
 struct Span {
   int lo, len, s0, s1;
 };
-template <int KS> __device__ __forceinline__ Span span_of(const Params& p, int b) {
+template <int KS> __device__ __forceinline__ Span span_of(const Params& p, int len) {
   Span z;
-  int len = p.seq_len[b];
   // out of range (reported by plan_steps): nothing is visible
   if (len < 0 || len > 0x7fffffff - KS || (int64_t)len > (int64_t)p.max_pages * p.page_size) len = 0;
   z.len = len;
@@ -80,6 +79,12 @@ template <int KS> __device__ __forceinline__ Span span_of(const Params& p, int b
   return z;
 }
 
+// a * b / c of non-negative numbers; 64-bit division takes some 100 instructions, so short lists go without
+__device__ __forceinline__ int64_t mul_div(int64_t a, int b, int64_t c) {
+  if (a * b <= 0xffffffffll && c <= 0xffffffffll) return (uint32_t)(a * b) / (uint32_t)c;
+  return a * b / c;
+}
+
 // How T steps are cut: n groups, group g = steps [T g / n, T (g + 1) / n), of which the last ns * tail are
 // ns tails. Piece j of group g (0: its head) is piece g (1 + ns) + j of the list.
 struct Cut {
@@ -87,18 +92,25 @@ struct Cut {
   int n, ns, tail;
   __device__ __forceinline__ Cut(int64_t steps, int W, int tails) : T(steps) {
     n = T < W ? (int)T : W;
-    tail = tails > 0 && n > 0 ? (int)(T / n / TAIL) : 0;
+    tail = tails > 0 && n > 0 ? (int)(mul_div(T, 1, n) / TAIL) : 0;
     ns = tail >= MIN_TAIL ? tails : 0;
   }
-  __device__ __forceinline__ int64_t group(int g) const { return T * g / n; }
+  __device__ __forceinline__ int64_t group(int g) const { return mul_div(T, g, n); }
   __device__ __forceinline__ int64_t first(int g, int j) const {
     return j == 0 ? group(g) : group(g + 1) - (int64_t)(ns - j + 1) * tail;
   }
-  __device__ __forceinline__ int piece_of(int64_t step) const {
-    const int g = (int)(((step + 1) * n + T - 1) / T) - 1;
-    if (ns == 0) return g;
-    const int64_t back = group(g + 1) - 1 - step;
-    return g * (1 + ns) + (back < (int64_t)ns * tail ? ns - (int)(back / tail) : 0);
+  // the piece that holds a step, and that piece's first step
+  __device__ __forceinline__ int piece_of(int64_t step, int64_t& begin) const {
+    // the largest g with T g / n <= step, that is g < (step + 1) n / T
+    int g = (int)mul_div(step + 1, n, T);
+    if (g >= n || group(g) > step) --g;
+    int j = 0;
+    if (ns > 0) {
+      const int64_t back = group(g + 1) - 1 - step;
+      if (back < (int64_t)ns * tail) j = ns - (int)back / tail;
+    }
+    begin = first(g, j);
+    return g * (1 + ns) + j;
   }
 };
 
@@ -184,11 +196,21 @@ __device__ __forceinline__ float lse_of(float m, float l) {
   return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-// Position of a worker in the step list.
+// Position of a worker in the step list. Lane i holds the length of sequence `base` + i.
 struct Cursor {
   int b, u, s;      // sequence, unit of the sequence (KV head x tile), step
+  int base, lens;
   Span z;
 };
+template <int KS>
+__device__ __forceinline__ void enter(const Params& p, Cursor& c) {
+  if (c.b >= c.base + 32) {
+    c.base = c.b;
+    const int i = c.b + (threadIdx.x & 31);
+    c.lens = i < p.B ? p.seq_len[i] : 0;
+  }
+  c.z = span_of<KS>(p, __shfl_sync(0xffffffffu, c.lens, c.b - c.base));
+}
 // To the next step; true when it starts another unit.
 template <int KS>
 __device__ __forceinline__ bool advance(const Params& p, Cursor& c) {
@@ -197,7 +219,7 @@ __device__ __forceinline__ bool advance(const Params& p, Cursor& c) {
     c.u = 0;
     do {
       if (++c.b >= p.B) return true;
-      c.z = span_of<KS>(p, c.b);
+      enter<KS>(p, c);
     } while (c.z.s1 <= c.z.s0);
   }
   c.s = c.z.s0;
@@ -221,9 +243,10 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
   const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) {
-    const Span z = span_of<KS>(p, b);
+    const int len = p.seq_len[b];
+    const Span z = span_of<KS>(p, len);
     mine += (z.s1 - z.s0) * units;
-    if (blockIdx.x == 0 && z.len != p.seq_len[b]) report(CAST_DEV_BAD_LAYOUT);
+    if (blockIdx.x == 0 && z.len != len) report(CAST_DEV_BAD_LAYOUT);
   }
   int64_t inc = mine;
 #pragma unroll
@@ -243,7 +266,7 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
     int64_t at = sums[tid];
     for (int b = b0; b < b1; ++b) {
       p.cum[b] = at;
-      const Span z = span_of<KS>(p, b);
+      const Span z = span_of<KS>(p, p.seq_len[b]);
       at += (z.s1 - z.s0) * units;
     }
     if (tid == 0) p.cum[p.B] = sums[NT];
@@ -267,19 +290,19 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
   // the run of sequences that holds step `begin`: the last thread whose first step is <= begin
   int cnt = 0;
   for (int i = 0; i < NT / 32; ++i) cnt += __popc(__ballot_sync(0xffffffffu, sums[i * 32 + lane] <= begin));
-  int b = (cnt - 1) * per;
+  c.b = (cnt - 1) * per;
+  c.base = c.b - 32;
   int64_t at = sums[cnt - 1];
   while (true) {
-    c.z = span_of<KS>(p, b);
+    enter<KS>(p, c);
     const int64_t n = (c.z.s1 - c.z.s0) * units;
     if (begin < at + n) break;
     at += n;
-    ++b;
+    ++c.b;
   }
-  c.b = b;
   const int steps = c.z.s1 - c.z.s0;
-  c.u = (int)((begin - at) / steps);
-  c.s = c.z.s0 + (int)((begin - at) % steps);
+  c.u = (int)mul_div(begin - at, 1, steps);
+  c.s = c.z.s0 + (int)(begin - at - (int64_t)c.u * steps);
   return wk;
 }
 
@@ -756,14 +779,15 @@ __global__ void __launch_bounds__(JOIN_NT) decode_join_kernel(const Params p) {
   int w0 = 0, w1 = 0, first = 0, r = 0;      // pieces of the row's unit
   const bool split = have && c1 != c0;
   if (split) {
-    const int64_t steps = (c1 - c0) / units;
+    const int64_t steps = mul_div(c1 - c0, 1, units);
     const int hr = hq % p.G, u = (hq / p.G) * p.tiles + hr / p.rows;
     r = hr % p.rows;
     const int64_t us = c0 + u * steps;
     const Cut cut(T_all, p.W, p.ns);
-    w0 = cut.piece_of(us);
-    w1 = cut.piece_of(us + steps - 1);
-    first = 2 * w0 + (cut.first(w0 / (1 + cut.ns), w0 % (1 + cut.ns)) == us ? 0 : 1);
+    int64_t begin, last;
+    w0 = cut.piece_of(us, begin);
+    w1 = cut.piece_of(us + steps - 1, last);
+    first = 2 * w0 + (begin == us ? 0 : 1);
   }
   float M = -INFINITY, L = 0.f, acc[DV];
 #pragma unroll
