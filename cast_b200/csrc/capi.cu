@@ -1117,6 +1117,8 @@ cudaError_t launch_append(papp::Args& a, const papp::Layers& ly, bool vec, int n
     a.np = a.h / v;
     a.X = a.np + (a.D - 2 * a.h) / v;
   }
+  const uint64_t heads = (uint64_t)a.H_q + 2 * a.H_kv;
+  a.heads_inv = (uint32_t)((0x100000000ull + heads - 1) / heads);
   int64_t blocks;
   if (a.keep) {
     a.tok = papp::MAX_TOK;
@@ -1206,6 +1208,7 @@ int cast_paged_append(int n_layers, void* const* pages_kv, const void* const* ne
       table_stride < 0 || keep_stride < 0 || n_freq < 0 || 2 * n_freq > D)
     return CAST_ERR_SHAPE;
   if (D > papp::MAX_D) return CAST_ERR_HEAD_DIM;
+  if (H_kv > papp::MAX_HEADS || H_q > papp::MAX_HEADS) return CAST_ERR_SHAPE;
   if (total > 0x7fffffffLL) return CAST_ERR_SHAPE;
   if ((q == nullptr) != (q_out == nullptr)) return CAST_ERR_NULL;
   if (q && (n_layers != 1 || keep || H_q < 1 || n_freq == 0)) return CAST_ERR_SHAPE;

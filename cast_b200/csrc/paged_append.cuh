@@ -10,11 +10,12 @@
 // are 32-bit, and each result is rounded once to the cache's type.
 //
 // Bound: memory traffic for prompts (2 bytes moved per byte of k, v and q), the latency of the chain
-// length -> table entry -> store for a few rows. One CTA takes `tok` consecutive rows (4 when that still
+// length -> table entry -> store for a few rows. One CTA takes `tok` consecutive rows (2 when that still
 // gives every SM several CTAs, else 1) and all their heads, so an angle is computed once per row and
 // shared by H_q + H_kv heads through shared memory. Thread (x, y): x = 16-byte pieces of a head, y steps
 // over (row, head); a piece of the first half travels with its partner of the second half, so both
-// results come from one thread's registers. Loads are issued before the angles are computed.
+// results come from one thread's registers. The first loads are issued before the row's sequence, page
+// and angles are known.
 #pragma once
 
 #include "common.cuh"
@@ -23,10 +24,11 @@ namespace cast {
 namespace papp {
 
 constexpr int NT = 256;
-constexpr int MAX_TOK = 4;      // rows per CTA
+constexpr int MAX_TOK = 2;      // rows per CTA
 constexpr int MAX_D = 256;
+constexpr int MAX_HEADS = 4096;
 constexpr int MAXL = 64;        // layers per launch
-constexpr int UNROLL = 4;       // (row, head) items a thread loads before it stores the first
+constexpr int UNROLL = 3;       // (row, head) items a thread loads before it stores the first
 
 struct Layers {
   const void* src[MAXL][2];   // new K, V rows
@@ -37,6 +39,7 @@ struct Args {
   int H_kv, H_q, D, h;                 // h = rotated pairs per head
   int interleaved, tok;
   int X, np;                           // pieces per head and thread column count; paired pieces
+  uint32_t heads_inv;                  // ceil(2^32 / (H_q + 2 H_kv)): i / heads for i < 2^16
   float rope_scale;
   int num_pages, page_size, max_pages, B;
   int64_t table_stride;
@@ -67,14 +70,14 @@ __device__ __forceinline__ int find_seq(const int32_t* cu_q, int B, int64_t t) {
   return c == 0 ? -1 : lo + c - 1;
 }
 
-// cos and sin of pos * freq: quadrant and remainder in 64 bits, the remainder's functions in 32.
+// cos and sin of pos * freq: quarter turns and the rest of one in 64 bits, the rest's functions in 32
+// (sincospif: within half a quarter turn it needs no further reduction).
 __device__ __forceinline__ void cos_sin(int pos, float freq, float& c, float& s) {
+  constexpr double kTwoOverPi = 0.63661977236758134308;
   const double th = (double)pos * (double)freq;
-  const double n = rint(th * 0.63661977236758134308);                       // 2 / pi
-  double r = fma(n, -1.57079632679489661923, th);                           // pi / 2, high part
-  r = fma(n, -6.123233995736766e-17, r);                                    // and what it leaves of pi / 2
+  const double n = rint(th * kTwoOverPi);
   float sr, cr;
-  sincosf((float)r, &sr, &cr);
+  sincospif(0.5f * (float)fma(th, kTwoOverPi, -n), &sr, &cr);
   const int k = (int)((long long)n & 3);
   c = (k & 1) ? sr : cr;
   s = (k & 1) ? cr : sr;
@@ -82,8 +85,13 @@ __device__ __forceinline__ void cos_sin(int pos, float freq, float& c, float& s)
   if (k >= 2) s = -s;
 }
 
+__device__ __forceinline__ float2 pair_to_f(__nv_bfloat162 x) { return __bfloat1622float2(x); }
+__device__ __forceinline__ float2 pair_to_f(__half2 x) { return __half22float2(x); }
+__device__ __forceinline__ void pair_from_f(__nv_bfloat162& x, float a, float b) { x = __floats2bfloat162_rn(a, b); }
+__device__ __forceinline__ void pair_from_f(__half2& x, float a, float b) { x = __floats2half2_rn(a, b); }
+
 // VEC consecutive elements as one memory access
-template <typename T, int VEC> struct Piece {
+template <typename T, int VEC> struct alignas(VEC * sizeof(T)) Piece {
   T x[VEC];
 };
 template <typename T, int VEC>
@@ -99,6 +107,33 @@ __device__ __forceinline__ void store_piece(T* p, const Piece<T, VEC>& r) {
   else *p = r.x[0];
 }
 
+// The pairs (a[e], b[e]) turned by (c[e], s[e]), rounded once; 16-bit types convert two values at a time.
+template <typename T, int VEC>
+__device__ __forceinline__ void turn(Piece<T, VEC>& a, Piece<T, VEC>& b, const float* c, const float* s) {
+  if constexpr (sizeof(T) == 2 && VEC == 8) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2* pa = reinterpret_cast<T2*>(a.x);
+    T2* pb = reinterpret_cast<T2*>(b.x);
+    const float4 c0 = *reinterpret_cast<const float4*>(c), c1 = *reinterpret_cast<const float4*>(c + 4);
+    const float4 s0 = *reinterpret_cast<const float4*>(s), s1 = *reinterpret_cast<const float4*>(s + 4);
+    const float2 cc[4] = {{c0.x, c0.y}, {c0.z, c0.w}, {c1.x, c1.y}, {c1.z, c1.w}};
+    const float2 ss[4] = {{s0.x, s0.y}, {s0.z, s0.w}, {s1.x, s1.y}, {s1.z, s1.w}};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 u = pair_to_f(pa[e]), v = pair_to_f(pb[e]);
+      pair_from_f(pa[e], u.x * cc[e].x - v.x * ss[e].x, u.y * cc[e].y - v.y * ss[e].y);
+      pair_from_f(pb[e], v.x * cc[e].x + u.x * ss[e].x, v.y * cc[e].y + u.y * ss[e].y);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float u = Elem<T>::to_f(a.x[e]), v = Elem<T>::to_f(b.x[e]);
+      a.x[e] = Elem<T>::from_f(u * c[e] - v * s[e]);
+      b.x[e] = Elem<T>::from_f(v * c[e] + u * s[e]);
+    }
+  }
+}
+
 struct RowMeta {
   int64_t row;      // source row, -1: nothing to do
   int64_t dk, dv;   // element offset of the destination row (head 0) in the K / V pages
@@ -106,7 +141,7 @@ struct RowMeta {
 };
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(NT) append_kernel(const Args a, const __grid_constant__ Layers ly) {
+__global__ void __launch_bounds__(NT, 4) append_kernel(const Args a, const __grid_constant__ Layers ly) {
   __shared__ RowMeta meta[MAX_TOK];
   __shared__ __align__(16) float cs[MAX_TOK][MAX_D / 2], sn[MAX_TOK][MAX_D / 2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -117,7 +152,7 @@ __global__ void __launch_bounds__(NT) append_kernel(const Args a, const __grid_c
   T* dv = static_cast<T*>(ly.dst[l][1]);
   const T* q = static_cast<const T*>(a.q);
   T* qo = static_cast<T*>(a.q_out);
-  const int X = a.X, Y = NT / X;
+  const int X = a.X, Y = NT / X;           // threads beyond X * Y have no items
   const int x = tid % X, y = tid / X;
   const bool half_pair = x < a.np;           // a second piece belongs to this one
   const bool scalar_pairs = a.interleaved && VEC == 1;
@@ -139,8 +174,68 @@ __global__ void __launch_bounds__(NT) append_kernel(const Args a, const __grid_c
     }
     rounds = (n_acc + a.tok - 1) / a.tok;
   }
+  const int items = a.tok * heads;
+  const bool busy = y < Y;
+  Piece<T, VEC> pa[UNROLL], pb[UNROLL];
+  // source row of the CTA's k-th row; without lists it is known before the sequence it belongs to is
+  auto row_of = [&](int k) -> int64_t {
+    if (accept) return meta[k].row;
+    const int64_t r = (int64_t)blockIdx.x * a.tok + k;
+    return r < a.total ? r : -1;
+  };
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int i = i0 + u * Y + y;
+      if (!busy || i >= items) continue;
+      const int k = (int)__umulhi((uint32_t)i, a.heads_inv), hd = i - k * heads;
+      const int64_t row = row_of(k);
+      if (row < 0) continue;
+      const bool is_v = hd >= a.H_q + a.H_kv;
+      const T* src;
+      if (hd < a.H_q) src = q + row * a.sq_t + hd * a.sq_h;
+      else if (!is_v) src = sk + row * a.sk_t + (hd - a.H_q) * a.sk_h;
+      else src = sv + row * a.sv_t + (hd - a.H_q - a.H_kv) * a.sv_h;
+      pa[u] = load_piece<T, VEC>(src + (is_v ? voff_a : off_a));
+      if (half_pair) pb[u] = load_piece<T, VEC>(src + (is_v ? voff_b : off_b));
+    }
+  };
+  auto store = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int i = i0 + u * Y + y;
+      if (!busy || i >= items) continue;
+      const int k = (int)__umulhi((uint32_t)i, a.heads_inv), hd = i - k * heads;
+      const RowMeta m = meta[k];
+      if (m.row < 0) continue;
+      const bool is_v = hd >= a.H_q + a.H_kv;
+      T* dst;
+      if (hd < a.H_q) dst = qo + m.row * a.so_t + hd * a.so_h;
+      else if (!is_v) dst = dk + m.dk + (hd - a.H_q) * a.pk_h;
+      else dst = dv + m.dv + (hd - a.H_q - a.H_kv) * a.pv_h;
+      if (!is_v) {
+        if (a.interleaved && VEC > 1) {
+          if (x * VEC < 2 * a.h) {
+            const float* c = cs[k] + x * (VEC / 2);
+            const float* s = sn[k] + x * (VEC / 2);
+#pragma unroll
+            for (int e = 0; e + 1 < VEC; e += 2) {
+              const float u0 = Elem<T>::to_f(pa[u].x[e]), u1 = Elem<T>::to_f(pa[u].x[e + 1]);
+              pa[u].x[e] = Elem<T>::from_f(u0 * c[e / 2] - u1 * s[e / 2]);
+              pa[u].x[e + 1] = Elem<T>::from_f(u1 * c[e / 2] + u0 * s[e / 2]);
+            }
+          }
+        } else if (half_pair) {
+          turn<T, VEC>(pa[u], pb[u], cs[k] + x * VEC, sn[k] + x * VEC);
+        }
+      }
+      store_piece<T, VEC>(dst + (is_v ? voff_a : off_a), pa[u]);
+      if (half_pair) store_piece<T, VEC>(dst + (is_v ? voff_b : off_b), pb[u]);
+    }
+  };
   for (int rd = 0; rd < rounds; ++rd) {
     if (rd > 0) __syncthreads();             // the previous round's rows are done with meta, cs and sn
+    if (!accept) load(0);
     for (int k = warp; k < a.tok; k += NT / 32) {
       int b, j;
       int64_t row;
@@ -199,79 +294,21 @@ __global__ void __launch_bounds__(NT) append_kernel(const Args a, const __grid_c
       }
     }
     __syncthreads();
-    const int items = a.tok * heads;
-    bool first = true;
-    for (int i0 = y; first || i0 < items; i0 += Y * UNROLL) {
-      Piece<T, VEC> pa[UNROLL], pb[UNROLL];
-      const T* src[UNROLL];
-      if (y < Y) {
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-          const int i = i0 + u * Y;
-          src[u] = nullptr;
-          if (i >= items) continue;
-          const int k = i / heads, hd = i - k * heads;
-          const int64_t row = meta[k].row;
-          if (row < 0) continue;
-          const bool is_v = hd >= a.H_q + a.H_kv;
-          if (hd < a.H_q) src[u] = q + row * a.sq_t + hd * a.sq_h;
-          else if (!is_v) src[u] = sk + row * a.sk_t + (hd - a.H_q) * a.sk_h;
-          else src[u] = sv + row * a.sv_t + (hd - a.H_q - a.H_kv) * a.sv_h;
-          pa[u] = load_piece<T, VEC>(src[u] + (is_v ? voff_a : off_a));
-          if (half_pair) pb[u] = load_piece<T, VEC>(src[u] + (is_v ? voff_b : off_b));
-        }
-      }
-      if (first) {
-        // the angles of this round's rows, while the first loads are under way
-        for (int e = tid; e < a.tok * a.h; e += NT) {
-          const int k = e / a.h, i = e - k * a.h;
-          if (meta[k].row < 0) continue;
-          float c, s;
-          cos_sin(meta[k].pos, a.inv_freq[i], c, s);
-          cs[k][i] = c * a.rope_scale;
-          sn[k][i] = s * a.rope_scale;
-        }
-        __syncthreads();
-        first = false;
-      }
-      if (y < Y) {
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-          if (src[u] == nullptr) continue;
-          const int i = i0 + u * Y;
-          const int k = i / heads, hd = i - k * heads;
-          const bool is_v = hd >= a.H_q + a.H_kv;
-          T* dst;
-          if (hd < a.H_q) dst = qo + meta[k].row * a.so_t + hd * a.so_h;
-          else if (!is_v) dst = dk + meta[k].dk + (hd - a.H_q) * a.pk_h;
-          else dst = dv + meta[k].dv + (hd - a.H_q - a.H_kv) * a.pv_h;
-          if (!is_v) {
-            if (a.interleaved && VEC > 1) {
-              if (x * VEC < 2 * a.h) {
-                const float* c = cs[k] + x * (VEC / 2);
-                const float* s = sn[k] + x * (VEC / 2);
-#pragma unroll
-                for (int e = 0; e + 1 < VEC; e += 2) {
-                  const float u0 = Elem<T>::to_f(pa[u].x[e]), u1 = Elem<T>::to_f(pa[u].x[e + 1]);
-                  pa[u].x[e] = Elem<T>::from_f(u0 * c[e / 2] - u1 * s[e / 2]);
-                  pa[u].x[e + 1] = Elem<T>::from_f(u1 * c[e / 2] + u0 * s[e / 2]);
-                }
-              }
-            } else if (half_pair) {
-              const float* c = cs[k] + x * VEC;
-              const float* s = sn[k] + x * VEC;
-#pragma unroll
-              for (int e = 0; e < VEC; ++e) {
-                const float u0 = Elem<T>::to_f(pa[u].x[e]), u1 = Elem<T>::to_f(pb[u].x[e]);
-                pa[u].x[e] = Elem<T>::from_f(u0 * c[e] - u1 * s[e]);
-                pb[u].x[e] = Elem<T>::from_f(u1 * c[e] + u0 * s[e]);
-              }
-            }
-          }
-          store_piece<T, VEC>(dst + (is_v ? voff_a : off_a), pa[u]);
-          if (half_pair) store_piece<T, VEC>(dst + (is_v ? voff_b : off_b), pb[u]);
-        }
-      }
+    if (accept) load(0);
+    // the angles of this round's rows, while the first loads are under way
+    for (int e = tid; e < a.tok * a.h; e += NT) {
+      const int k = e / a.h, i = e - k * a.h;
+      if (meta[k].row < 0) continue;
+      float c, s;
+      cos_sin(meta[k].pos, a.inv_freq[i], c, s);
+      cs[k][i] = c * a.rope_scale;
+      sn[k][i] = s * a.rope_scale;
+    }
+    __syncthreads();
+    store(0);
+    for (int i0 = Y * UNROLL; i0 < items; i0 += Y * UNROLL) {
+      load(i0);
+      store(i0);
     }
   }
 }
