@@ -65,6 +65,7 @@ struct AttnParams {
   const int32_t* page_table;
   int64_t table_stride;
   int num_pages, page_size, box;
+  int bm;   // rows of a query tile of the tensor-core kernel: 128 / G * G
 };
 
 // Key tiles of one sequence: the whole range for the regular layout, the

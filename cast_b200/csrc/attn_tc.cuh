@@ -1,4 +1,4 @@
-// Tensor-core (tcgen05 / TMEM / TMA) ragged tree attention for 16-bit inputs, D = 128.
+// Tensor-core (tcgen05 / TMEM / TMA) ragged tree attention for 16-bit inputs, D = 128 (paged: also 64).
 //
 // Work unit (one CTA, one per SM): sequence b, KV head h, up to two 128-row
 // query tiles of the G*P_b rows of that head group (row r = pack token r / G,
@@ -135,14 +135,19 @@ __device__ __forceinline__ int ranked_sequence(const AttnParams& p, int rank, in
 // page (the 128-byte swizzle goes by the shared-memory address, so boxes of fewer than 8 rows land as
 // one of 128 would put them). The producer warp's lanes issue them side by side, each from a table
 // entry that it read while the previous tile was under way.
+// Head groups that do not divide 128 (paged only) take p.bm = 128 / G * G rows of each query tile: the
+// copies leave the last rows of the tile's shared memory as they were, the MMAs compute on them, and
+// nothing is written for them (a row of S, P or O depends on its own row of Q alone). DH = 64 uses the
+// first of a tile's two 64-column panels.
 enum KvLayout { kRagged = 0, kStore = 1, kPaged = 2 };
-template <bool BF16, int LAYOUT>
+template <bool BF16, int LAYOUT, int DH = 128>
 __global__ void __launch_bounds__(NT, 1)
 attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKp,
                const __grid_constant__ CUtensorMap tmVp) {
   using namespace tc;
   constexpr bool STORE = LAYOUT != kRagged;   // prefix tiles and pack tiles come from different tensors
+  constexpr int D = DH, PANELS = DH / 64;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* sAnc = reinterpret_cast<uint64_t*>(smem + SMEM_ANC);
@@ -185,14 +190,15 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
     return;
   }
   const int G = p.G;
+  const int bm = LAYOUT == kPaged ? p.bm : BM;   // rows of a query tile
   const int rows = G * m.P;
   if (p.tail_only) {   // only the sequence's partial last 256-row block (the CTA-pair launch runs the rest)
     if (rows % (QT * BM) == 0) return;
     mblk = rows / (QT * BM);
   }
-  const int r_base = mblk * (QT * BM);
+  const int r_base = mblk * (QT * bm);
   if (r_base >= rows) return;
-  const int n_qt = (rows - r_base > BM) ? 2 : 1;
+  const int n_qt = (rows - r_base > bm) ? 2 : 1;
   const int nkeys = m.S + m.P;
   // Key tiles of this CTA. Regular layout: keys [k_begin, k_end) of concat(prefix, pack),
   // tile j at key k_begin + 128 j. Store layout: tiles [t_begin, t_begin + n_kt) of the
@@ -253,7 +259,7 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
   }
   if (warp == 0) tmem_alloc(smem_u32(&tmem_base_sh), 512);
   const int i_lo = r_base / G;
-  const int i_hi = min(m.P - 1, (r_base + QT * BM - 1) / G);
+  const int i_hi = min(m.P - 1, (r_base + QT * bm - 1) / G);
   // the pack's parents up to the last token of the block, staged for the bitset walks
   int* sPar = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(sAnc) + (size_t)anc_tokens(G) * p.W * sizeof(uint64_t));
   const bool stage = has_pack_tile && p.anc_words == nullptr && p.W <= kStageParentMaxW;
@@ -271,13 +277,13 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
   const uint32_t ring = smem_u32(smem + (is_k ? SMEM_K : SMEM_V));
   const CUtensorMap* m_reg = is_k ? &tmK : &tmV;
   const CUtensorMap* m_pack = is_k ? &tmKp : &tmVp;
-  // Paged prefix: lane l copies half l & 1 of boxes l / 2, l / 2 + 16, ...; the table entry of its first
-  // box in tile j + 1 is read while tile j is being copied.
+  // Paged prefix: lane l copies panel l % PANELS of boxes l / PANELS, + 32 / PANELS, ...; the table entry of
+  // its first box in tile j + 1 is read while tile j is being copied.
   auto page_at = [&](int n) -> int {
     return n < m.S ? p.page_table[b * p.table_stride + n / p.page_size] : -1;
   };
   int next_page = -1;
-  if (LAYOUT == kPaged && (warp == 0 || warp == 2)) next_page = page_at(t_begin * BN + (lane >> 1) * p.box);
+  if (LAYOUT == kPaged && (warp == 0 || warp == 2)) next_page = page_at(t_begin * BN + lane / PANELS * p.box);
   // one 128-key tile (two 64-column halves) into ring slot j % NST
   auto issue_tile = [&](int j) {
     const uint32_t dst = ring + (j % NST) * TILE_BYTES, bar = smem_u32(&full[j % NST]);
@@ -285,21 +291,21 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
     if (LAYOUT == kPaged && t < nt_pre) {
       const int n0 = t * BN, boxes = (min(BN, m.S - n0) + p.box - 1) / p.box;
       int page = next_page;
-      next_page = page_at(n0 + BN + (lane >> 1) * p.box);
-      if (elect_one()) mbar_expect_tx(bar, boxes * p.box * 256);
+      next_page = page_at(n0 + BN + lane / PANELS * p.box);
+      if (elect_one()) mbar_expect_tx(bar, boxes * p.box * (PANELS * 128));
       __syncwarp();
-      for (int i = lane >> 1; i < boxes; i += 16) {
+      for (int i = lane / PANELS; i < boxes; i += 32 / PANELS) {
         const int n = n0 + i * p.box;
-        if (i >= 16) page = page_at(n);
+        if (i >= 32 / PANELS) page = page_at(n);
         if (page < 0 || page >= p.num_pages) {
           report(CAST_DEV_BAD_LAYOUT);
           page = p.num_pages;          // past the last page: the copy fills zeros
         }
-        tma_load_4d(dst + (lane & 1) * HALF_BYTES + i * p.box * 128, m_reg, (lane & 1) * 64, n % p.page_size, h, page, bar);
+        tma_load_4d(dst + lane % PANELS * HALF_BYTES + i * p.box * 128, m_reg, lane % PANELS * 64, n % p.page_size, h, page, bar);
       }
     } else if (elect_one()) {
-      mbar_expect_tx(bar, TILE_BYTES);
-      for (int hf = 0; hf < 2; ++hf) {
+      mbar_expect_tx(bar, PANELS * HALF_BYTES);
+      for (int hf = 0; hf < PANELS; ++hf) {
         if constexpr (STORE) {
           if (t < nt_pre) tma_load_4d(dst + hf * HALF_BYTES, m_reg, hf * 64, t * BN, h, b, bar);
           else tma_load_3d(dst + hf * HALF_BYTES, m_pack, hf * 64, h, m.q0 + (t - nt_pre) * BN, bar);
@@ -315,10 +321,10 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
   const int n_early = min(NST, n_kt);
   if (warp == 0 || warp == 2) {
     if (is_k && elect_one()) {
-      mbar_expect_tx(qf, n_qt * TILE_BYTES);
+      mbar_expect_tx(qf, n_qt * bm * (PANELS * 128));
       for (int q = 0; q < n_qt; ++q) {
-        const int tok = m.q0 + (r_base + q * BM) / G;
-        for (int hf = 0; hf < 2; ++hf)
+        const int tok = m.q0 + (r_base + q * bm) / G;
+        for (int hf = 0; hf < PANELS; ++hf)
           tma_load_3d(smem_u32(smem + SMEM_Q + q * TILE_BYTES + hf * HALF_BYTES), &tmQ, hf * 64, h * G, tok, qf);
       }
     }
@@ -400,8 +406,8 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
         tile_keys(j, n0, klim);
         if (n0 < m.S && n0 + BN > m.S) {
           uint8_t* vt = smem + SMEM_V + s * TILE_BYTES;
-          for (int e = lane; e < (n0 + BN - m.S) * 16; e += 32) {
-            const int r = m.S - n0 + (e >> 4), c = e & 15;
+          for (int e = lane; e < (n0 + BN - m.S) * (8 * PANELS); e += 32) {
+            const int r = m.S - n0 + e / (8 * PANELS), c = e % (8 * PANELS);
             *reinterpret_cast<uint4*>(vt + (c >> 3) * HALF_BYTES + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
@@ -501,7 +507,7 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
       const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t S_t = tmem + lane_off + q * 128;
       const uint32_t O_t = tmem + lane_off + 256 + q * 128;
-      const int r = r_base + (dual ? 0 : q * BM) + t;
+      const int r = r_base + (dual ? 0 : q * bm) + t;
       // key tiles of this warpgroup: all of them, or every other one in dual mode
       const int n_steps = dual ? (n_kt + 1 - q) / 2 : n_kt;
       const int li = min(r / G, m.P - 1) - i_lo;
@@ -570,7 +576,7 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
         // lazy correction of O (rows whose max grew by more than 2^8); PV_{j-1} is complete
         if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) {
+          for (int cc = 0; cc < D / 32; ++cc) {
             tmem_ld32(O_t + cc * 32, v);
             tmem_ld_wait();
 #pragma unroll
@@ -622,7 +628,7 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
         }
       };
       if (done) {
-        const bool store = r < rows;
+        const bool store = r < rows && (LAYOUT != kPaged || t < bm);
         const int i = min(r / G, m.P - 1), hq = h * G + r % G;
         const int64_t tq = m.q0 + i;
         if (p.n_split == 1) {
@@ -630,7 +636,7 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
           using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
           T* out = static_cast<T*>(p.out) + tq * p.so_m + (int64_t)hq * p.so_h;
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) {
+          for (int cc = 0; cc < D / 32; ++cc) {
             load_o(cc);
             uint32_t pk[16];
 #pragma unroll
@@ -646,7 +652,7 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
           const int64_t slot = ((int64_t)split * p.total_q + tq) * p.H_q + hq;
           float* O = p.ws_o + slot * D;
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) {
+          for (int cc = 0; cc < D / 32; ++cc) {
             load_o(cc);
             if (store) {
               float4* dst = reinterpret_cast<float4*>(O + cc * 32);

@@ -52,7 +52,7 @@ struct SimtPlan {
   size_t ws_bytes;
 };
 
-SimtPlan plan_simt(int B, int total_q, int H_q, int H_kv, int D, int max_pack, int max_kv, int sms) {
+SimtPlan plan_simt(int B, int total_q, int H_q, int H_kv, int D, int max_pack, int max_kv, int sms, int min_tiles = 4) {
   SimtPlan pl;
   const int G = H_q / H_kv;
   pl.m_tiles = (G * max_pack + simt::BM - 1) / simt::BM;
@@ -64,7 +64,7 @@ SimtPlan plan_simt(int B, int total_q, int H_q, int H_kv, int D, int max_pack, i
   const int kv = max_kv > 0 ? max_kv : 1;
   int chunk = ((kv + simt::BN - 1) / simt::BN) * simt::BN;
   int n_split = 1;
-  while (base * n_split < target && chunk > 4 * simt::BN) {
+  while (base * n_split < target && chunk > min_tiles * simt::BN) {
     n_split *= 2;
     chunk = (((kv + n_split - 1) / n_split + simt::BN - 1) / simt::BN) * simt::BN;
   }
@@ -136,11 +136,34 @@ TcPlan plan_tc(int B, int total_q, int H_q, int H_kv, int max_pack, int max_kv, 
   return pl;
 }
 
+// Fewest key tiles of a chunk of the paged layout.
+constexpr int kPagedMinTiles = 4, kPagedMinTilesSimt = 1;
+
 // Store layout: key tiles per sequence are ceil(S/128) + ceil(P/128); plan on
 // that tile count (chunks stay whole numbers of tiles).
 TcPlan plan_tc_store(int B, int total_q, int H_q, int H_kv, int max_pack, int max_prefix, int sms) {
   const int tiles = (max_prefix + tca::BN - 1) / tca::BN + (max_pack + tca::BN - 1) / tca::BN;
   return plan_tc(B, total_q, H_q, H_kv, max_pack, tiles * tca::BN, sms);
+}
+
+// Paged layout: tiles as in the store layout, any head group up to 128 (128 / G * G rows per query tile).
+TcPlan plan_tc_paged(int B, int total_q, int H_q, int H_kv, int D, int max_pack, int max_prefix, int sms) {
+  TcPlan pl;
+  const int G = H_q / H_kv, bm = tca::BM / G * G;
+  pl.m_blocks = std::max(1, (G * max_pack + tca::QT * bm - 1) / (tca::QT * bm));
+  pl.W = std::max(1, (max_pack + 63) / 64);
+  const long long base = (long long)B * H_kv * pl.m_blocks;
+  const long long target = 2LL * (sms > 0 ? sms : 148);
+  const int tiles = std::max(1, (max_prefix + tca::BN - 1) / tca::BN + (max_pack + tca::BN - 1) / tca::BN);
+  int ct = tiles, n_split = 1;
+  while (base * n_split < target && ct > kPagedMinTiles) {
+    n_split *= 2;
+    ct = (tiles + n_split - 1) / n_split;
+  }
+  pl.n_split = (tiles + ct - 1) / ct;
+  pl.chunk = ct * tca::BN;
+  pl.ws_bytes = pl.n_split > 1 ? (size_t)pl.n_split * total_q * H_q * (D + 2) * sizeof(float) : 0;
+  return pl;
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
@@ -155,12 +178,12 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
 }
 
-// 3-D map over a [rows, heads, 128] 16-bit tensor: box = 64 dims x `box_heads` x `box_rows`, 128-byte swizzle.
+// 3-D map over a [rows, heads, D] 16-bit tensor: box = 64 dims x `box_heads` x `box_rows`, 128-byte swizzle.
 bool make_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int heads, int64_t s_row, int64_t s_head,
-              int box_heads, int box_rows) {
+              int box_heads, int box_rows, int D = 128) {
   auto enc = tensor_map_encoder();
   if (!enc) return false;
-  cuuint64_t dims[3] = {128, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
   cuuint64_t strides[2] = {(cuuint64_t)s_head * 2, (cuuint64_t)s_row * 2};
   cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
   cuuint32_t es[3] = {1, 1, 1};
@@ -196,12 +219,12 @@ bool make_store_map(CUtensorMap* map, const void* base, int dtype, int batch, in
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// 4-D map over pages [num_pages, heads, page_size, 128]: box = 64 dims x `box` rows of one head of one page.
-bool make_pages_map(CUtensorMap* map, const void* base, int dtype, int num_pages, int heads, int page_size,
+// 4-D map over pages [num_pages, heads, page_size, D]: box = 64 dims x `box` rows of one head of one page.
+bool make_pages_map(CUtensorMap* map, const void* base, int dtype, int num_pages, int heads, int page_size, int D,
                     int64_t s_p, int64_t s_h, int64_t s_r, int box_rows) {
   auto enc = tensor_map_encoder();
   if (!enc) return false;
-  cuuint64_t dims[4] = {128, (cuuint64_t)page_size, (cuuint64_t)heads, (cuuint64_t)num_pages};
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page_size, (cuuint64_t)heads, (cuuint64_t)num_pages};
   cuuint64_t strides[3] = {(cuuint64_t)s_r * 2, (cuuint64_t)s_h * 2, (cuuint64_t)s_p * 2};
   cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
   cuuint32_t es[4] = {1, 1, 1, 1};
@@ -211,7 +234,7 @@ bool make_pages_map(CUtensorMap* map, const void* base, int dtype, int num_pages
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int LAYOUT>
+template <int LAYOUT, int DH = 128>
 int launch_tc_maps(AttnParams& p, const TcPlan& pl, int dtype, cudaStream_t st, const CUtensorMap& mq,
                    const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mkp, const CUtensorMap& mvp,
                    bool combine = true) {
@@ -220,17 +243,18 @@ int launch_tc_maps(AttnParams& p, const TcPlan& pl, int dtype, cudaStream_t st, 
   p.m_tiles = pl.m_blocks;
   p.W = pl.W;
   {
-    const long long last = ((long long)p.G * p.max_pack) % (tca::QT * tca::BM);
-    p.tail_last = (last > 0 && last <= tca::BM) ? 1 : 0;
+    const int bm = LAYOUT == tca::kPaged ? p.bm : tca::BM;
+    const long long last = ((long long)p.G * p.max_pack) % (tca::QT * bm);
+    p.tail_last = (last > 0 && last <= bm) ? 1 : 0;
   }
   const size_t smem = tca::smem_bytes(p.G, pl.W);
   dim3 grid(p.tail_only ? 1 : pl.m_blocks, p.B * p.H_kv, pl.n_split);
   if (dtype == CAST_BF16) {
-    cudaFuncSetAttribute(tca::attn_tc_kernel<true, LAYOUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    tca::attn_tc_kernel<true, LAYOUT><<<grid, tca::NT, smem, st>>>(p, mq, mk, mv, mkp, mvp);
+    cudaFuncSetAttribute(tca::attn_tc_kernel<true, LAYOUT, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    tca::attn_tc_kernel<true, LAYOUT, DH><<<grid, tca::NT, smem, st>>>(p, mq, mk, mv, mkp, mvp);
   } else {
-    cudaFuncSetAttribute(tca::attn_tc_kernel<false, LAYOUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    tca::attn_tc_kernel<false, LAYOUT><<<grid, tca::NT, smem, st>>>(p, mq, mk, mv, mkp, mvp);
+    cudaFuncSetAttribute(tca::attn_tc_kernel<false, LAYOUT, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    tca::attn_tc_kernel<false, LAYOUT, DH><<<grid, tca::NT, smem, st>>>(p, mq, mk, mv, mkp, mvp);
   }
   if (cudaGetLastError() != cudaSuccess) return CAST_ERR_LAUNCH;
   if (combine && pl.n_split > 1) {
@@ -1338,9 +1362,9 @@ size_t cast_tree_attn_paged_workspace_size(int dtype, int B, int total_q, int H_
   if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return 0;
   if (B <= 0 || total_q <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || (D != 64 && D != 128)) return 0;
   const int sms = sm_count();
-  const size_t ws = plan_simt(B, total_q, H_q, H_kv, D, max_pack, max_prefix + max_pack, sms).ws_bytes;
-  if (dtype == CAST_F32 || D != 128 || 128 % (H_q / H_kv) != 0) return ws;
-  return std::max(ws, plan_tc_store(B, total_q, H_q, H_kv, max_pack, max_prefix, sms).ws_bytes);
+  const size_t ws = plan_simt(B, total_q, H_q, H_kv, D, max_pack, max_prefix + max_pack, sms, kPagedMinTilesSimt).ws_bytes;
+  if (dtype == CAST_F32 || H_q / H_kv > tca::BM) return ws;
+  return std::max(ws, plan_tc_paged(B, total_q, H_q, H_kv, D, max_pack, max_prefix, sms).ws_bytes);
 }
 
 int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_pack,
@@ -1395,10 +1419,10 @@ int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_p
   p.num_pages = num_pages; p.page_size = page_size;
   p.wait_ns = g_pipeline_wait_ns.load(std::memory_order_relaxed);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  bool tensor = dtype != CAST_F32 && D == 128 && 128 % G == 0 && g_tc_kernel.load(std::memory_order_relaxed) >= 0;
+  bool tensor = dtype != CAST_F32 && G <= tca::BM && g_tc_kernel.load(std::memory_order_relaxed) >= 0;
   for (const int64_t* t : {sq, skp, svp, so}) tensor = tensor && t[0] % 8 == 0 && t[1] % 8 == 0;
   if (!tensor) {
-    const SimtPlan pl = plan_simt(B, total_q, H_q, H_kv, D, max_pack, p.max_kv, sms);
+    const SimtPlan pl = plan_simt(B, total_q, H_q, H_kv, D, max_pack, p.max_kv, sms, kPagedMinTilesSimt);
     if (pl.ws_bytes > 0) {
       if (!workspace || workspace_bytes < pl.ws_bytes || !aligned(workspace, 16)) return CAST_ERR_WORKSPACE;
       p.ws_o = static_cast<float*>(workspace);
@@ -1413,20 +1437,22 @@ int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_p
   p.store_mode = 1;
   p.box = tca::BN;
   while (page_size % p.box != 0) p.box /= 2;   // gcd(page_size, 128)
-  const TcPlan pl = plan_tc_store(B, total_q, H_q, H_kv, max_pack, max_prefix, sms);
+  p.bm = tca::BM / G * G;
+  const TcPlan pl = plan_tc_paged(B, total_q, H_q, H_kv, D, max_pack, max_prefix, sms);
   if (pl.ws_bytes > 0) {
     if (!workspace || workspace_bytes < pl.ws_bytes || !aligned(workspace, 16)) return CAST_ERR_WORKSPACE;
     p.ws_o = static_cast<float*>(workspace);
     p.ws_ml = p.ws_o + (size_t)pl.n_split * total_q * H_q * D;
   }
   CUtensorMap mq, mks, mvs, mkp, mvp;
-  if (!make_map(&mq, q, dtype, total_q, H_q, sq[0], sq[1], G, tca::BM / G) ||
-      !make_pages_map(&mks, k_pages, dtype, num_pages, H_kv, page_size, sp[0], sp[1], sp[2], p.box) ||
-      !make_pages_map(&mvs, v_pages, dtype, num_pages, H_kv, page_size, sp[0], sp[1], sp[2], p.box) ||
-      !make_map(&mkp, k_pack, dtype, total_q, H_kv, skp[0], skp[1], 1, tca::BN) ||
-      !make_map(&mvp, v_pack, dtype, total_q, H_kv, svp[0], svp[1], 1, tca::BN))
+  if (!make_map(&mq, q, dtype, total_q, H_q, sq[0], sq[1], G, tca::BM / G, D) ||
+      !make_pages_map(&mks, k_pages, dtype, num_pages, H_kv, page_size, D, sp[0], sp[1], sp[2], p.box) ||
+      !make_pages_map(&mvs, v_pages, dtype, num_pages, H_kv, page_size, D, sp[0], sp[1], sp[2], p.box) ||
+      !make_map(&mkp, k_pack, dtype, total_q, H_kv, skp[0], skp[1], 1, tca::BN, D) ||
+      !make_map(&mvp, v_pack, dtype, total_q, H_kv, svp[0], svp[1], 1, tca::BN, D))
     return CAST_ERR_LAUNCH;
-  return launch_tc_maps<tca::kPaged>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp);
+  return D == 128 ? launch_tc_maps<tca::kPaged, 128>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp)
+                  : launch_tc_maps<tca::kPaged, 64>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp);
 }
 
 }  // extern "C"

@@ -646,16 +646,22 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
       h0 = h * p.G + (cc.u % p.tiles) * p.rows;
       nrow = min(p.rows, h * p.G + p.G - h0);
       const float* q = static_cast<const float*>(p.q) + (int64_t)cc.b * p.sq_b + (int64_t)h0 * p.sq_h;
-      __syncwarp();
+      float x[GT][D / 32];                 // all loads before the first store
 #pragma unroll
       for (int a = 0; a < GT; ++a) {
-        for (int d = lane; d < D; d += 32) sq[warp][a][d] = a < nrow ? q[(int64_t)a * p.sq_h + d] : 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) x[a][i] = a < nrow ? q[(int64_t)a * p.sq_h + i * 32 + lane] : 0.f;
+        slope[a] = (p.slopes != nullptr && a < nrow) ? p.slopes[h0 + a] : 0.f;
         m[a] = -INFINITY;
         l[a] = 0.f;
-        slope[a] = (p.slopes != nullptr && a < nrow) ? p.slopes[h0 + a] : 0.f;
 #pragma unroll
         for (int i = 0; i < DV; ++i) o[a][i] = 0.f;
       }
+      __syncwarp();
+#pragma unroll
+      for (int a = 0; a < GT; ++a)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) sq[warp][a][i * 32 + lane] = x[a][i];
     }
     cp_wait<NST - 2>();
     __syncwarp();

@@ -21,21 +21,23 @@ and a verify round of draft trees, whose accepted rows are appended for every la
 A length or page id out of range is skipped on the device and reported by ``_lib.device_error()``.
 """
 import struct
+from functools import lru_cache
 
 import torch
 
 from . import _lib
-from .tree_attn import _DTYPES, _kernel_ready, _prep
+from .tree_attn import _DTYPES
 
 
 # The device and the stream of a call as plain integers: the objects of torch.cuda.current_stream() take 2 us a call,
 # a tenth of what a one-token step has.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _launch(index, fn, name, *args):
     """Calls a C entry point on the current stream of device `index` (its last argument), with that device current."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         code = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -74,6 +76,45 @@ def _pages(k_pages, v_pages, name):
     if v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype is not dtype or v_pages.device != dev:
         raise ValueError(f"{name}: K and V pages need one shape, one dtype, one device and the same strides")
     return shape, stride, dtype, dev
+
+
+def _aligned(stride, ptr):
+    """What the attention kernels take: dim stride 1, row / head strides multiples of 4, a 16-byte aligned base."""
+    return stride[2] == 1 and stride[0] % 4 == 0 and stride[1] % 4 == 0 and ptr % 16 == 0
+
+
+def _input(t):
+    """t as the kernels take it (a copy where it is not), its strides and its address."""
+    stride, ptr = t.stride(), t.data_ptr()
+    if not _aligned(stride, ptr):
+        t = t.contiguous()
+        stride, ptr = t.stride(), t.data_ptr()
+    return t, stride, ptr
+
+
+def _output(out, q, shape, dtype, dev):
+    """The given or a new output, its strides and its address."""
+    if out is None:
+        out = torch.empty_like(q)
+        return out, out.stride(), out.data_ptr()
+    stride, ptr = out.stride(), out.data_ptr()
+    if out.shape != shape or out.dtype is not dtype or out.device != dev or not _aligned(stride, ptr):
+        raise ValueError("out must be like q: dim stride 1, row/head strides multiple of 4, 16-byte aligned base")
+    return out, stride, ptr
+
+
+@lru_cache(maxsize=256)
+def _decode_bytes(index, *args):
+    """cast_paged_decode_workspace_size on device `index` (its SM count plays a part)."""
+    with torch.cuda.device(index):
+        return _lib.lib().cast_paged_decode_workspace_size(*args)
+
+
+def _tree_bytes(index, *args):
+    if _current_device() == index:
+        return _lib.lib().cast_tree_attn_paged_workspace_size(*args)
+    with torch.cuda.device(index):
+        return _lib.lib().cast_tree_attn_paged_workspace_size(*args)
 
 
 def _workspace(workspace, n, dev):
@@ -209,11 +250,8 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     seq_len = _i32(seq_len, dev, "seq_len", B)
     if window < 0 or not (softcap == 0.0 or 1e-6 <= softcap <= 1e30):
         raise ValueError("decode_attention_paged: window must not be negative, softcap 0 or 1e-6 to 1e30")
-    q = _prep(q)
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != shape or out.dtype is not dtype or out.device != dev or not _kernel_ready(out):
-        raise ValueError("out must be like q: dim stride 1, row/head strides multiple of 4, 16-byte aligned base")
+    q, sq, p_q = _input(q)
+    out, so, p_out = _output(out, q, shape, dtype, dev)
     p_slopes = p_lse = None
     if alibi_slopes is not None:
         if alibi_slopes.dtype is not torch.float32 or alibi_slopes.device != dev or not alibi_slopes.is_contiguous():
@@ -225,12 +263,11 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
         if lse.shape != (B, H_q) or lse.dtype is not torch.float32 or lse.device != dev or not lse.is_contiguous():
             raise ValueError("lse must be a contiguous float32 [B, H_q]")
         p_lse = lse.data_ptr()
-    L, code = _lib.lib(), _DTYPES[dtype]
-    n = L.cast_paged_decode_workspace_size(code, B, H_q, H_kv, D)
+    code = _DTYPES[dtype]
+    n = _decode_bytes(dev.index, code, B, H_q, H_kv, D)
     workspace = _workspace(workspace, n, dev)
-    sq, so = q.stride(), out.stride()
-    _launch(dev.index, L.cast_paged_decode_attn, "cast_paged_decode_attn", q.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), out.data_ptr(), p_lse, code, _I7(sq[0], sq[1], sp[0], sp[1], sp[2], so[0], so[1]),
+    _launch(dev.index, _lib.lib().cast_paged_decode_attn, "cast_paged_decode_attn", p_q, k_pages.data_ptr(),
+            v_pages.data_ptr(), p_out, p_lse, code, _I7(sq[0], sq[1], sp[0], sp[1], sp[2], so[0], so[1]),
             table.data_ptr(), table.stride(0), width, seq_len.data_ptr(), B, H_q, H_kv, D, num_pages, ps,
             0.0 if sm_scale is None else sm_scale, softcap, window, p_slopes,
             None if workspace is None else workspace.data_ptr(), n)
@@ -244,8 +281,8 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
 
     q: [total_q, H_q, D]; request b's prefix is keys [0, prefix_len[b]) of its pages; k_pack / v_pack:
     [total_q, H_kv, D], this pass's keys and values in pack order. Output, masks and conventions as
-    varlen_tree_attention. bfloat16 / float16 with D = 128 and H_q / H_kv dividing 128 run on the tensor cores
-    straight from the pages, whatever their size; float32 and other head shapes on the exact CUDA-core kernel.
+    varlen_tree_attention. bfloat16 / float16 with H_q / H_kv <= 128 run on the tensor cores straight from the
+    pages, whatever their size; float32 on the exact CUDA-core kernel. D 64 or 128.
     max_pack / max_prefix bound pack_len and prefix_len; given, the call reads nothing back to the host.
     """
     (num_pages, H_kv, ps, D), sp, dtype, dev = _pages(k_pages, v_pages, "varlen_tree_attention_paged")
@@ -266,11 +303,10 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
         max_pack = int(pack_len.max().item()) if B > 0 else 0
     if max_prefix is None:
         max_prefix = int(prefix_len.max().item()) if B > 0 else 0
-    q, k_pack, v_pack = _prep(q), _prep(k_pack), _prep(v_pack)
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != shape or out.dtype is not dtype or out.device != dev or not _kernel_ready(out):
-        raise ValueError("out must be like q: dim stride 1, row/head strides multiple of 4, 16-byte aligned base")
+    q, sq, p_q = _input(q)
+    k_pack, sk, p_k = _input(k_pack)
+    v_pack, sv, p_v = _input(v_pack)
+    out, so, p_out = _output(out, q, shape, dtype, dev)
     anc_ptr, wpr, par_ptr = None, 0, None
     if ancestor_mask is not None:
         anc = ancestor_mask
@@ -283,12 +319,11 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
     else:
         parent = _i32(parent, dev, "parent", total_q)
         par_ptr = parent.data_ptr()
-    L, code = _lib.lib(), _DTYPES[dtype]
-    n = L.cast_tree_attn_paged_workspace_size(code, B, total_q, H_q, H_kv, D, max_pack, max_prefix)
+    code = _DTYPES[dtype]
+    n = _tree_bytes(dev.index, code, B, total_q, H_q, H_kv, D, max_pack, max_prefix)
     workspace = _workspace(workspace, n, dev)
-    sq, sk, sv, so = q.stride(), k_pack.stride(), v_pack.stride(), out.stride()
-    _launch(dev.index, L.cast_tree_attn_paged_fwd, "cast_tree_attn_paged_fwd", q.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), k_pack.data_ptr(), v_pack.data_ptr(), out.data_ptr(), code,
+    _launch(dev.index, _lib.lib().cast_tree_attn_paged_fwd, "cast_tree_attn_paged_fwd", p_q, k_pages.data_ptr(),
+            v_pages.data_ptr(), p_k, p_v, p_out, code,
             _I11(sq[0], sq[1], sp[0], sp[1], sp[2], sk[0], sk[1], sv[0], sv[1], so[0], so[1]), table.data_ptr(),
             table.stride(0), width, cu_q.data_ptr(), prefix_len.data_ptr(), pack_len.data_ptr(), anc_ptr, wpr, par_ptr,
             B, total_q, num_pages, ps, H_q, H_kv, D, 0.0 if sm_scale is None else sm_scale, max_pack, max_prefix,

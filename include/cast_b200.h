@@ -464,9 +464,8 @@ size_t cast_paged_decode_workspace_size(int dtype, int B, int H_q, int H_kv, int
  * ancestor conventions are those of cast_tree_attn_fwd. strides[11] = q (row, head),
  * pages (page, head, row; keys and values alike), k_pack, v_pack, out (row, head);
  * multiples of 4 elements, page strides multiples of 16 bytes, bases 16-byte aligned.
- * CAST_BF16 / CAST_F16 with D = 128, H_q / H_kv dividing 128 and strides that are
- * multiples of 8 run on the tensor cores, everything else (CAST_F32, exact; D = 64)
- * on the CUDA cores. Keys past prefix_len[b] in a page are never part of the result.
+ * CAST_BF16 / CAST_F16 with H_q / H_kv <= 128 and strides that are multiples of 8
+ * run on the tensor cores, everything else (CAST_F32, exact) on the CUDA cores. Keys past prefix_len[b] in a page are never part of the result.
  * max_prefix bounds prefix_len[b] (a longer one is reported as CAST_DEV_BAD_LAYOUT).
  */
 int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_pack,

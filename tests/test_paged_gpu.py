@@ -485,9 +485,13 @@ def test_tree_words_rows_without_keys_and_rows_behind(cuda, dtype):
 
 
 def test_tree_equals_the_store_form(cuda):
-    S, P = [0, 128, 257, 1000], [64, 1, 129, 300]
+    # 40 sequences x 8 KV heads are 320 units, above the two per SM up to which either launch plan splits the keys (the
+    # plans cut small launches differently, and partial sums of other cuts round differently): the same tiles in the
+    # same order, so the same bits
+    rng = np.random.default_rng(25)
+    S, P = [0, 128, 257, 1000] + rng.integers(0, 300, 36).tolist(), [64, 1, 129, 300] + rng.integers(1, 40, 36).tolist()
     c, q, kp, vp, parents, cu = _tree_inputs(cuda, 25, S, P, 32, 8, 128, 16, torch.bfloat16)
-    ks = torch.zeros(4, 8, 1024, 128, dtype=torch.bfloat16, device=cuda)
+    ks = torch.zeros(40, 8, 1024, 128, dtype=torch.bfloat16, device=cuda)
     vs = torch.zeros_like(ks)
     for b, s in enumerate(S):
         ks[b, :, :s], vs[b, :, :s] = c.rows(c.k[0], b, 0, s).transpose(0, 1), c.rows(c.v[0], b, 0, s).transpose(0, 1)
