@@ -1162,18 +1162,17 @@ int decode_rows(int dtype, int G) {
   return std::min(G, dtype == CAST_F32 ? 8 : 32);
 }
 
-// Workspace: first steps [B + 1] int64, then the partials of two units per piece of the step list.
+// Workspace: the partials of two units per piece of the step list.
 struct DecodeLayout {
   int rows, workers;
-  size_t o, ml, total;
+  size_t ml, total;
 };
-DecodeLayout decode_layout(int dtype, int B, int G, int D, int sms) {
+DecodeLayout decode_layout(int dtype, int G, int D, int sms) {
   DecodeLayout l;
   l.rows = decode_rows(dtype, G);
   l.workers = sms * pdec::CTAS_PER_SM * pdec::NW;
   const size_t slots = 2 * (size_t)l.workers * (1 + pdec::NS) * l.rows;
-  l.o = align256((size_t)(B + 1) * sizeof(int64_t));
-  l.ml = l.o + align256(slots * D * sizeof(float));
+  l.ml = align256(slots * D * sizeof(float));
   l.total = l.ml + align256(slots * 2 * sizeof(float));
   return l;
 }
@@ -1292,7 +1291,7 @@ size_t cast_paged_decode_workspace_size(int dtype, int B, int H_q, int H_kv, int
   if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return 0;
   if (B <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || (D != 64 && D != 128)) return 0;
   const int sms = sm_count();
-  return decode_layout(dtype, B, H_q / H_kv, D, sms > 0 ? sms : 148).total;
+  return decode_layout(dtype, H_q / H_kv, D, sms > 0 ? sms : 148).total;
 }
 
 int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pages, void* out, float* lse, int dtype,
@@ -1316,7 +1315,7 @@ int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pag
   const int sms = sm_count();
   if (sms <= 0) return CAST_ERR_DEVICE;
   const int G = H_q / H_kv;
-  const DecodeLayout lay = decode_layout(dtype, B, G, D, sms);
+  const DecodeLayout lay = decode_layout(dtype, G, D, sms);
   if (!workspace || workspace_bytes < lay.total || !aligned(workspace, 256)) return CAST_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
   pdec::Params p{};
@@ -1346,8 +1345,7 @@ int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pag
   // a unit has about (pieces / units) partials; eight of them are one warp's round in the join
   p.join_warps = 1;
   while (p.join_warps < 8 && (int64_t)p.join_warps * 8 * B * H_kv * p.tiles < (int64_t)p.W * (1 + p.ns)) p.join_warps *= 2;
-  p.cum = reinterpret_cast<int64_t*>(ws);
-  p.ws_o = reinterpret_cast<float*>(ws + lay.o);
+  p.ws_o = reinterpret_cast<float*>(ws);
   p.ws_ml = reinterpret_cast<float*>(ws + lay.ml);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t err;

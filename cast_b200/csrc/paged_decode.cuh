@@ -61,7 +61,6 @@ struct Params {
   int W, ns;                                       // groups of steps at most; tails per group (0 or NS)
   float* ws_o;                                     // [2 W (1 + ns)][rows][D]
   float* ws_ml;                                    // [2 W (1 + ns)][rows][2]: running maximum (log2 units), sum
-  int64_t* cum;                                    // [B + 1] first step of each sequence
 };
 
 // Visible keys [lo, len) of sequence b and the steps that cover them (step s = keys [s KS, (s + 1) KS)).
@@ -226,19 +225,12 @@ __device__ __forceinline__ bool advance(const Params& p, Cursor& c) {
   return true;
 }
 
-// What this warp does: its piece of the list and the cursor at the piece's first step.
-struct Work {
-  int piece;        // -1: nothing
-  int steps;
-  Cursor c;
-};
-// The block sums its threads' runs of sequences, scans the sums and finds the sequence that holds the
-// piece's first step. CTA 0 writes each sequence's first step for the join kernel.
-template <int KS>
-__device__ __forceinline__ Work plan_steps(const Params& p) {
-  __shared__ int64_t sums[NT + 1];
+// First step of every sequence, by a block of THREADS: thread t owns the run of `per` sequences from t * per
+// and sums[t] is the run's first step; sums[THREADS] = T.
+template <int KS, int THREADS>
+__device__ __forceinline__ int scan_steps(const Params& p, int64_t* sums, int64_t* wsum, bool check) {
   const int tid = threadIdx.x, lane = tid & 31;
-  const int per = (p.B + NT - 1) / NT;
+  const int per = (p.B + THREADS - 1) / THREADS;
   const int64_t units = (int64_t)p.H_kv * p.tiles;
   const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
   int64_t mine = 0;
@@ -246,7 +238,7 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
     const int len = p.seq_len[b];
     const Span z = span_of<KS>(p, len);
     mine += (z.s1 - z.s0) * units;
-    if (blockIdx.x == 0 && z.len != len) report(CAST_DEV_BAD_LAYOUT);
+    if (check && z.len != len) report(CAST_DEV_BAD_LAYOUT);
   }
   int64_t inc = mine;
 #pragma unroll
@@ -254,23 +246,28 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
     const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += x;
   }
-  __shared__ int64_t wsum[NW];
   if (lane == 31) wsum[tid >> 5] = inc;
   __syncthreads();
   int64_t before = 0;
   for (int i = 0; i < (tid >> 5); ++i) before += wsum[i];
   sums[tid] = before + inc - mine;
-  if (tid == NT - 1) sums[NT] = before + inc;
+  if (tid == THREADS - 1) sums[THREADS] = before + inc;
   __syncthreads();
-  if (blockIdx.x == 0) {
-    int64_t at = sums[tid];
-    for (int b = b0; b < b1; ++b) {
-      p.cum[b] = at;
-      const Span z = span_of<KS>(p, p.seq_len[b]);
-      at += (z.s1 - z.s0) * units;
-    }
-    if (tid == 0) p.cum[p.B] = sums[NT];
-  }
+  return per;
+}
+
+// What this warp does: its piece of the list and the cursor at the piece's first step.
+struct Work {
+  int piece;        // -1: nothing
+  int steps;
+  Cursor c;
+};
+template <int KS>
+__device__ __forceinline__ Work plan_steps(const Params& p) {
+  __shared__ int64_t sums[NT + 1], wsum[NW];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int64_t units = (int64_t)p.H_kv * p.tiles;
+  const int per = scan_steps<KS, NT>(p, sums, wsum, blockIdx.x == 0);
   const Cut cut(sums[NT], p.W, p.ns);
   Work wk;
   Cursor& c = wk.c;
@@ -769,32 +766,39 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
 // without a visible key become 0 (lse -inf).
 template <typename T, int D>
 __global__ void __launch_bounds__(JOIN_NT) decode_join_kernel(const Params p) {
-  constexpr int DV = D / 32, NB = 8;
+  constexpr int DV = D / 32, NB = 8, KS = step_keys<T, D>();
   __shared__ float part[JOIN_NT / 32][D];
   __shared__ float2 part_ml[JOIN_NT / 32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ int64_t sums[JOIN_NT + 1], wsum[JOIN_NT / 32];
+  // which partials: from the lengths alone, while the workers still run
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = scan_steps<KS, JOIN_NT>(p, sums, wsum, false);
   const int jw = p.join_warps, sub = warp % jw;
   const int64_t row = (int64_t)blockIdx.x * (JOIN_NT / 32 / jw) + warp / jw;
   const bool have = row < (int64_t)p.B * p.H_q;
   const int b = have ? (int)(row / p.H_q) : 0, hq = have ? (int)(row % p.H_q) : 0;
-  const int64_t T_all = p.cum[p.B];
-  const int64_t c0 = p.cum[b], c1 = p.cum[b + 1];
   const int units = p.H_kv * p.tiles;
   T* out = static_cast<T*>(p.out) + (int64_t)b * p.so_b + (int64_t)hq * p.so_h;
   int w0 = 0, w1 = 0, first = 0, r = 0;      // pieces of the row's unit
-  const bool split = have && c1 != c0;
+  const Span z = span_of<KS>(p, p.seq_len[b]);
+  const int steps = z.s1 - z.s0;
+  const bool split = have && steps > 0;
   if (split) {
-    const int64_t steps = mul_div(c1 - c0, 1, units);
+    int64_t c0 = sums[b / per];
+    for (int i = b / per * per; i < b; ++i) {
+      const Span y = span_of<KS>(p, p.seq_len[i]);
+      c0 += (int64_t)(y.s1 - y.s0) * units;
+    }
     const int hr = hq % p.G, u = (hq / p.G) * p.tiles + hr / p.rows;
     r = hr % p.rows;
-    const int64_t us = c0 + u * steps;
-    const Cut cut(T_all, p.W, p.ns);
+    const int64_t us = c0 + (int64_t)u * steps;
+    const Cut cut(sums[JOIN_NT], p.W, p.ns);
     int64_t begin, last;
     w0 = cut.piece_of(us, begin);
     w1 = cut.piece_of(us + steps - 1, last);
     first = 2 * w0 + (begin == us ? 0 : 1);
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float M = -INFINITY, L = 0.f, acc[DV];
 #pragma unroll
   for (int i = 0; i < DV; ++i) acc[i] = 0.f;

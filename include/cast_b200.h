@@ -446,7 +446,7 @@ int cast_paged_append(int n_layers, void* const* pages_kv, const void* const* ne
  * strides multiples of 16 bytes, bases 16-byte aligned. CAST_F32, CAST_BF16 or
  * CAST_F16, D 64 or 128. The lengths are not read on the host. Two launches; the
  * workspace (256-byte aligned, cast_paged_decode_workspace_size() bytes) needs no
- * initial value and does not depend on the lengths.
+ * initial value; its size depends on H_q / H_kv and D alone.
  */
 int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pages, void* out, float* lse, int dtype,
                            const int64_t* strides, const int32_t* page_table, int64_t table_stride, int max_pages,

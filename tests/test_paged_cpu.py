@@ -71,7 +71,7 @@ def test_decode_argument_checks(L):
 def test_decode_workspace_size(L):
     f = L.cast_paged_decode_workspace_size
     small, large = f(1, 1, 32, 8, 128), f(1, 4096, 32, 8, 128)
-    assert 0 < small < large and large - small <= 8 * 4096 + 256        # lengths play no part, B only by its offsets
+    assert 0 < small == large                                   # neither the lengths nor their number play a part
     assert f(1, 1, 30, 8, 128) == 0 and f(1, 1, 32, 8, 96) == 0 and f(3, 1, 32, 8, 128) == 0 and f(1, 0, 32, 8, 128) == 0
     assert cast_b200.decode_workspace_size(torch.bfloat16, 1, 32, 8, 128) == small
 
