@@ -162,6 +162,7 @@ attn_simt_kernel(const AttnParams p) {
   using namespace simt;
   constexpr int QS = qk_stride<D>();
   constexpr int CPT = D / 16;  // output columns per thread (4 or 8)
+  if constexpr (PAGED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(16) unsigned char smem_raw[];
   float* sQ = reinterpret_cast<float*>(smem_raw);
   float* sK = sQ + BM * QS;
@@ -387,33 +388,40 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const AttnParams p) {
   const int tiles_per_chunk = p.chunk / 128;
   const int nsplit = p.store_mode ? min(p.n_split, (seq_key_tiles(p, m.S, m.P, 128) + tiles_per_chunk - 1) / tiles_per_chunk)
                                   : min(p.n_split, (m.S + m.P + p.chunk - 1) / p.chunk);
+  // launched beside the kernel that writes the partials (paged layout): wait for it; else no wait
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // the chunks' maxima a lane each; then the chunks in order, the loads of eight under way at a time
+  const int64_t slot0 = (int64_t)t * p.H_q + hq, slots = (int64_t)p.total_q * p.H_q;
   float M = -INFINITY;
-  for (int z = 0; z < nsplit; ++z)
-    M = fmaxf(M, p.ws_ml[(((int64_t)z * p.total_q + t) * p.H_q + hq) * 2]);
+  for (int z = lane; z < nsplit; z += 32) M = fmaxf(M, p.ws_ml[(slot0 + z * slots) * 2]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
   const float m_use = (M == -INFINITY) ? 0.f : M;
   float L = 0.f;
-  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-  const int nv = p.D / 128 + (p.D % 128 ? 1 : 0);  // float4 groups per lane: D/128 (1 for D=64 uses half the lanes)
-  for (int z = 0; z < nsplit; ++z) {
-    const int64_t slot = ((int64_t)z * p.total_q + t) * p.H_q + hq;
-    const float w = exp2f(p.ws_ml[slot * 2] - m_use);
-    L += w * p.ws_ml[slot * 2 + 1];
-    const float* O = p.ws_o + slot * p.D;
-    for (int g = 0; g < nv; ++g) {
-      const int c = (g * 32 + lane) * 4;
-      if (c < p.D) {
-        const float4 x = *reinterpret_cast<const float4*>(O + c);
-        acc[g].x += w * x.x; acc[g].y += w * x.y; acc[g].z += w * x.z; acc[g].w += w * x.w;
-      }
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int c = lane * 4;                    // D <= 128: one float4 per lane (D = 64 uses half of them)
+  const bool has = c < p.D;
+  for (int z0 = 0; z0 < nsplit; z0 += 8) {
+    float2 ml[8];
+    float4 x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int z = min(z0 + k, nsplit - 1);
+      const int64_t slot = slot0 + z * slots;
+      ml[k] = *reinterpret_cast<const float2*>(p.ws_ml + slot * 2);
+      x[k] = has ? *reinterpret_cast<const float4*>(p.ws_o + slot * p.D + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (z0 + k >= nsplit) break;
+      const float w = exp2f(ml[k].x - m_use);
+      L += w * ml[k].y;
+      acc.x += w * x[k].x; acc.y += w * x[k].y; acc.z += w * x[k].z; acc.w += w * x[k].w;
     }
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;
   T* out = static_cast<T*>(p.out) + (int64_t)t * p.so_m + (int64_t)hq * p.so_h;
-  for (int g = 0; g < nv; ++g) {
-    const int c = (g * 32 + lane) * 4;
-    if (c < p.D)
-      store4<T>(out + c, make_float4(acc[g].x * inv, acc[g].y * inv, acc[g].z * inv, acc[g].w * inv));
-  }
+  if (has) store4<T>(out + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
 }
 
 }  // namespace cast

@@ -148,6 +148,7 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
   using namespace tc;
   constexpr bool STORE = LAYOUT != kRagged;   // prefix tiles and pack tiles come from different tensors
   constexpr int D = DH, PANELS = DH / 64;
+  if constexpr (LAYOUT == kPaged) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* sAnc = reinterpret_cast<uint64_t*>(smem + SMEM_ANC);

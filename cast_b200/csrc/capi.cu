@@ -75,6 +75,23 @@ SimtPlan plan_simt(int B, int total_q, int H_q, int H_kv, int D, int max_pack, i
   return pl;
 }
 
+// Sums up the key chunks' partials. `early` (paged layout): the kernel may start while the chunks' kernel
+// runs, and waits for it before it reads the partials; back to back the start of a small launch took 2.5 us.
+template <typename T>
+int launch_combine(const AttnParams& p, bool early, cudaStream_t st) {
+  const long long warps = (long long)p.total_q * p.H_q;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((warps * 32 + 255) / 256));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = early ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, attn_combine_kernel<T>, p) == cudaSuccess ? CAST_OK : CAST_ERR_LAUNCH;
+}
+
 template <typename T, bool PAGED = false>
 int launch_simt(AttnParams& p, const SimtPlan& pl, cudaStream_t st) {
   p.n_split = pl.n_split;
@@ -92,13 +109,7 @@ int launch_simt(AttnParams& p, const SimtPlan& pl, cudaStream_t st) {
     attn_simt_kernel<T, 64, PAGED><<<grid, simt::NT, smem, st>>>(p);
   }
   if (cudaGetLastError() != cudaSuccess) return CAST_ERR_LAUNCH;
-  if (pl.n_split > 1) {
-    const long long warps = (long long)p.total_q * p.H_q;
-    const int blocks = (int)((warps * 32 + 255) / 256);
-    attn_combine_kernel<T><<<blocks, 256, 0, st>>>(p);
-    if (cudaGetLastError() != cudaSuccess) return CAST_ERR_LAUNCH;
-  }
-  return CAST_OK;
+  return pl.n_split > 1 ? launch_combine<T>(p, PAGED, st) : CAST_OK;
 }
 
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
@@ -257,14 +268,9 @@ int launch_tc_maps(AttnParams& p, const TcPlan& pl, int dtype, cudaStream_t st, 
     tca::attn_tc_kernel<false, LAYOUT, DH><<<grid, tca::NT, smem, st>>>(p, mq, mk, mv, mkp, mvp);
   }
   if (cudaGetLastError() != cudaSuccess) return CAST_ERR_LAUNCH;
-  if (combine && pl.n_split > 1) {
-    const long long warps = (long long)p.total_q * p.H_q;
-    const int blocks = (int)((warps * 32 + 255) / 256);
-    if (dtype == CAST_BF16) attn_combine_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(p);
-    else attn_combine_kernel<__half><<<blocks, 256, 0, st>>>(p);
-    if (cudaGetLastError() != cudaSuccess) return CAST_ERR_LAUNCH;
-  }
-  return CAST_OK;
+  if (!combine || pl.n_split == 1) return CAST_OK;
+  constexpr bool early = LAYOUT == tca::kPaged;
+  return dtype == CAST_BF16 ? launch_combine<__nv_bfloat16>(p, early, st) : launch_combine<__half>(p, early, st);
 }
 
 // ---- fp32 through the tensor cores (three-term bf16 split) --------------------------
@@ -1159,7 +1165,8 @@ cudaError_t launch_append(papp::Args& a, const papp::Layers& ly, bool vec, int n
 
 // Query heads of one KV head that a worker takes together.
 int decode_rows(int dtype, int G) {
-  return std::min(G, dtype == CAST_F32 ? 8 : 32);
+  const int most = dtype == CAST_F32 ? 8 : 32, tiles = (G + most - 1) / most;
+  return (G + tiles - 1) / tiles;
 }
 
 // Workspace: the partials of two units per piece of the step list.
