@@ -52,7 +52,7 @@ struct SimtPlan {
   size_t ws_bytes;
 };
 
-SimtPlan plan_simt(int B, int total_q, int H_q, int H_kv, int D, int max_pack, int max_kv, int sms, int min_tiles = 4) {
+SimtPlan plan_simt(int B, int total_q, int H_q, int H_kv, int D, int max_pack, int max_kv, int sms, bool paged = false) {
   SimtPlan pl;
   const int G = H_q / H_kv;
   pl.m_tiles = (G * max_pack + simt::BM - 1) / simt::BM;
@@ -60,7 +60,9 @@ SimtPlan plan_simt(int B, int total_q, int H_q, int H_kv, int D, int max_pack, i
   pl.W = (max_pack + 63) / 64;
   if (pl.W < 1) pl.W = 1;
   const long long base = (long long)B * H_kv * pl.m_tiles;
-  const long long target = 2LL * (sms > 0 ? sms : 148);
+  // paged: finer chunks (a 64-key tile takes 2.7 us, an empty CTA next to nothing)
+  const long long target = (paged ? 8LL : 2LL) * (sms > 0 ? sms : 148);
+  const int min_tiles = paged ? 1 : 4;
   const int kv = max_kv > 0 ? max_kv : 1;
   int chunk = ((kv + simt::BN - 1) / simt::BN) * simt::BN;
   int n_split = 1;
@@ -147,9 +149,6 @@ TcPlan plan_tc(int B, int total_q, int H_q, int H_kv, int max_pack, int max_kv, 
   return pl;
 }
 
-// Fewest key tiles of a chunk of the paged layout.
-constexpr int kPagedMinTiles = 4, kPagedMinTilesSimt = 1;
-
 // Store layout: key tiles per sequence are ceil(S/128) + ceil(P/128); plan on
 // that tile count (chunks stay whole numbers of tiles).
 TcPlan plan_tc_store(int B, int total_q, int H_q, int H_kv, int max_pack, int max_prefix, int sms) {
@@ -158,18 +157,27 @@ TcPlan plan_tc_store(int B, int total_q, int H_q, int H_kv, int max_pack, int ma
 }
 
 // Paged layout: tiles as in the store layout, any head group up to 128 (128 / G * G rows per query tile).
+// A CTA has an SM for itself and some 14 us of set-up and epilogue besides its key tiles (1.8 us each, 1 us
+// with one query tile), so the keys are split only into as many chunks as run at once, and only where the
+// tiles saved outweigh the partials' way through memory (1 us + 8 us for 256 rows + 0.2 us a chunk). Measured, us, for n
+// chunks: 128 units of 17 tiles 49 (n = 1), 95 (2), 127 (4); 32 units of 17 tiles 45, 34, 28 (4), 38 (5); 8
+// units of 126 tiles 253, 138, 80 (4), 50 (8), 40 (16), 60 (24); 8 units of 5 one-tile blocks 15.6, 12.5 (5).
 TcPlan plan_tc_paged(int B, int total_q, int H_q, int H_kv, int D, int max_pack, int max_prefix, int sms) {
   TcPlan pl;
-  const int G = H_q / H_kv, bm = tca::BM / G * G;
-  pl.m_blocks = std::max(1, (G * max_pack + tca::QT * bm - 1) / (tca::QT * bm));
+  const int G = H_q / H_kv, bm = tca::BM / G * G, rows = G * max_pack;
+  pl.m_blocks = std::max(1, (rows + tca::QT * bm - 1) / (tca::QT * bm));
   pl.W = std::max(1, (max_pack + 63) / 64);
-  const long long base = (long long)B * H_kv * pl.m_blocks;
-  const long long target = 2LL * (sms > 0 ? sms : 148);
+  const long long base = std::max(1LL, (long long)B * H_kv * pl.m_blocks);
   const int tiles = std::max(1, (max_prefix + tca::BN - 1) / tca::BN + (max_pack + tca::BN - 1) / tca::BN);
-  int ct = tiles, n_split = 1;
-  while (base * n_split < target && ct > kPagedMinTiles) {
-    n_split *= 2;
-    ct = (tiles + n_split - 1) / n_split;
+  const int most = (int)std::max(1LL, std::min<long long>(tiles, (sms > 0 ? sms : 148) / base));
+  const float tile_us = rows > bm ? 1.8f : 1.0f;
+  const float split_us = 1.f + 8.f * std::min(rows, tca::QT * bm) / (tca::QT * bm);
+  int ct = tiles;
+  float best = tiles * tile_us;
+  for (int n = 2; n <= most; ++n) {
+    const int c = (tiles + n - 1) / n;
+    const float us = c * tile_us + split_us + 0.2f * n;
+    if (us < best) { best = us; ct = c; }
   }
   pl.n_split = (tiles + ct - 1) / ct;
   pl.chunk = ct * tca::BN;
@@ -1367,7 +1375,7 @@ size_t cast_tree_attn_paged_workspace_size(int dtype, int B, int total_q, int H_
   if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return 0;
   if (B <= 0 || total_q <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || (D != 64 && D != 128)) return 0;
   const int sms = sm_count();
-  const size_t ws = plan_simt(B, total_q, H_q, H_kv, D, max_pack, max_prefix + max_pack, sms, kPagedMinTilesSimt).ws_bytes;
+  const size_t ws = plan_simt(B, total_q, H_q, H_kv, D, max_pack, max_prefix + max_pack, sms, true).ws_bytes;
   if (dtype == CAST_F32 || H_q / H_kv > tca::BM) return ws;
   return std::max(ws, plan_tc_paged(B, total_q, H_q, H_kv, D, max_pack, max_prefix, sms).ws_bytes);
 }
@@ -1427,7 +1435,7 @@ int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_p
   bool tensor = dtype != CAST_F32 && G <= tca::BM && g_tc_kernel.load(std::memory_order_relaxed) >= 0;
   for (const int64_t* t : {sq, skp, svp, so}) tensor = tensor && t[0] % 8 == 0 && t[1] % 8 == 0;
   if (!tensor) {
-    const SimtPlan pl = plan_simt(B, total_q, H_q, H_kv, D, max_pack, p.max_kv, sms, kPagedMinTilesSimt);
+    const SimtPlan pl = plan_simt(B, total_q, H_q, H_kv, D, max_pack, p.max_kv, sms, true);
     if (pl.ws_bytes > 0) {
       if (!workspace || workspace_bytes < pl.ws_bytes || !aligned(workspace, 16)) return CAST_ERR_WORKSPACE;
       p.ws_o = static_cast<float*>(workspace);
