@@ -159,7 +159,7 @@ TcPlan plan_tc_store(int B, int total_q, int H_q, int H_kv, int max_pack, int ma
 // Paged layout: tiles as in the store layout, any head group up to 128 (128 / G * G rows per query tile).
 // A CTA has an SM for itself and some 14 us of set-up and epilogue besides its key tiles (1.8 us each, 1 us
 // with one query tile), so the keys are split only into as many chunks as run at once, and only where the
-// tiles saved outweigh the partials' way through memory (1 us + 8 us for 256 rows + 0.2 us a chunk). Measured, us, for n
+// tiles saved outweigh the partials' way through memory (0.05 us for each row above 60, 0.25 us a chunk). Measured, us, for n
 // chunks: 128 units of 17 tiles 49 (n = 1), 95 (2), 127 (4); 32 units of 17 tiles 45, 34, 28 (4), 38 (5); 8
 // units of 126 tiles 253, 138, 80 (4), 50 (8), 40 (16), 60 (24); 8 units of 5 one-tile blocks 15.6, 12.5 (5).
 TcPlan plan_tc_paged(int B, int total_q, int H_q, int H_kv, int D, int max_pack, int max_prefix, int sms) {
@@ -171,12 +171,12 @@ TcPlan plan_tc_paged(int B, int total_q, int H_q, int H_kv, int D, int max_pack,
   const int tiles = std::max(1, (max_prefix + tca::BN - 1) / tca::BN + (max_pack + tca::BN - 1) / tca::BN);
   const int most = (int)std::max(1LL, std::min<long long>(tiles, (sms > 0 ? sms : 148) / base));
   const float tile_us = rows > bm ? 1.8f : 1.0f;
-  const float split_us = 1.f + 8.f * std::min(rows, tca::QT * bm) / (tca::QT * bm);
+  const float split_us = std::max(0.5f, 0.05f * (std::min(rows, tca::QT * bm) - 60));
   int ct = tiles;
   float best = tiles * tile_us;
   for (int n = 2; n <= most; ++n) {
     const int c = (tiles + n - 1) / n;
-    const float us = c * tile_us + split_us + 0.2f * n;
+    const float us = c * tile_us + split_us + 0.25f * n;
     if (us < best) { best = us; ct = c; }
   }
   pl.n_split = (tiles + ct - 1) / ct;

@@ -46,22 +46,22 @@ def _launch(index, fn, name, *args):
         _lib.check(code, name)
 
 
-def _i32(t, dev, what, n=None):
-    """t as a contiguous int32 tensor on dev; n: the entries it must have."""
+def _i32(t, index, what, n=None):
+    """t as a contiguous int32 tensor on device `index`; n: the entries it must have."""
     if not isinstance(t, torch.Tensor):
         t = torch.as_tensor(t)
-    if t.dtype is not torch.int32 or t.device != dev or not t.is_contiguous():
-        t = t.to(device=dev, dtype=torch.int32).contiguous()
+    if t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
+        t = t.to(device=index, dtype=torch.int32).contiguous()
     if n is not None and t.numel() != n:
         raise ValueError(f"{what} must have {n} entries, not {tuple(t.shape)}")
     return t
 
 
-def _table(page_table, dev):
+def _table(page_table, index):
     if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
         raise ValueError("page_table must be a tensor [B, pages of a sequence]")
-    if page_table.dtype is not torch.int32 or page_table.device != dev or page_table.stride(1) != 1:
-        page_table = page_table.to(device=dev, dtype=torch.int32).contiguous()
+    if page_table.dtype is not torch.int32 or page_table.get_device() != index or page_table.stride(1) != 1:
+        page_table = page_table.to(device=index, dtype=torch.int32).contiguous()
     return page_table
 
 
@@ -69,13 +69,13 @@ def _pages(k_pages, v_pages, name):
     """Checks the pages of one layer: [num_pages, H_kv, page_size, D], K and V alike. Returns what they share."""
     if not k_pages.is_cuda:
         raise RuntimeError(f"cast_b200.{name} needs CUDA tensors (no CPU path)")
-    shape, stride, dtype, dev = k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.device
+    shape, stride, dtype, index = k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device()
     if len(shape) != 4 or stride[3] != 1 or dtype not in _DTYPES:
         raise ValueError(f"{name}: pages are [num_pages, H_kv, page_size, D] of float32, bfloat16 or float16, "
                          "dim stride 1")
-    if v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype is not dtype or v_pages.device != dev:
+    if v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype is not dtype or v_pages.get_device() != index:
         raise ValueError(f"{name}: K and V pages need one shape, one dtype, one device and the same strides")
-    return shape, stride, dtype, dev
+    return shape, stride, dtype, index
 
 
 def _aligned(stride, ptr):
@@ -92,13 +92,13 @@ def _input(t):
     return t, stride, ptr
 
 
-def _output(out, q, shape, dtype, dev):
+def _output(out, q, shape, dtype, index):
     """The given or a new output, its strides and its address."""
     if out is None:
         out = torch.empty_like(q)
         return out, out.stride(), out.data_ptr()
     stride, ptr = out.stride(), out.data_ptr()
-    if out.shape != shape or out.dtype is not dtype or out.device != dev or not _aligned(stride, ptr):
+    if out.shape != shape or out.dtype is not dtype or out.get_device() != index or not _aligned(stride, ptr):
         raise ValueError("out must be like q: dim stride 1, row/head strides multiple of 4, 16-byte aligned base")
     return out, stride, ptr
 
@@ -117,12 +117,12 @@ def _tree_bytes(index, *args):
         return _lib.lib().cast_tree_attn_paged_workspace_size(*args)
 
 
-def _workspace(workspace, n, dev):
-    """The caller's workspace where it is large enough and on dev, else a new one (None: nothing is needed)."""
+def _workspace(workspace, n, index):
+    """The caller's workspace where it is large enough and on device `index`, else a new one (None: nothing is needed)."""
     if n == 0:
         return None
-    if workspace is None or workspace.nbytes < n or workspace.data_ptr() % 256 or workspace.device != dev:
-        return torch.empty(n, dtype=torch.uint8, device=dev)
+    if workspace is None or workspace.nbytes < n or workspace.data_ptr() % 256 or workspace.get_device() != index:
+        return torch.empty(n, dtype=torch.uint8, device=index)
     return workspace
 
 
@@ -154,7 +154,7 @@ def append_paged(k_pages, v_pages, page_table, seq_len, k, v, cu_q=None, *, keep
         raise ValueError("append_paged: one K and one V of pages and of new rows per layer")
     if n == 0:
         return None
-    shape, sp, dtype, dev = _pages(kps[0], vps[0], "append_paged")
+    shape, sp, dtype, index = _pages(kps[0], vps[0], "append_paged")
     num_pages, H, ps, D = shape
     rows, sk, sv = ks[0].shape, ks[0].stride(), vs[0].stride()
     if len(rows) != 3 or rows[1] != H or rows[2] != D or sk[2] != 1 or sv[2] != 1:
@@ -163,58 +163,58 @@ def append_paged(k_pages, v_pages, page_table, seq_len, k, v, cu_q=None, *, keep
     for i in range(n):
         kp, vp, a, b = kps[i], vps[i], ks[i], vs[i]
         if i and (kp.shape != shape or vp.shape != shape or kp.stride() != sp or vp.stride() != sp
-                  or kp.dtype is not dtype or vp.dtype is not dtype or kp.device != dev or vp.device != dev):
+                  or kp.dtype is not dtype or vp.dtype is not dtype or kp.get_device() != index or vp.get_device() != index):
             raise ValueError("append_paged: every layer's pages need one shape, one dtype and the same strides")
-        if a.shape != rows or b.shape != rows or a.dtype is not dtype or b.dtype is not dtype or a.device != dev \
-                or b.device != dev:
+        if a.shape != rows or b.shape != rows or a.dtype is not dtype or b.dtype is not dtype or a.get_device() != index \
+                or b.get_device() != index:
             raise ValueError("append_paged: new rows are [total, H_kv, D] of the pages' dtype and device, dim stride 1")
         if i and (a.stride() != sk or b.stride() != sv):
             raise ValueError("append_paged: every layer's new rows need the same strides")
         pages += (kp.data_ptr(), vp.data_ptr())
         new += (a.data_ptr(), b.data_ptr())
     total = rows[0]
-    table = _table(page_table, dev)
+    table = _table(page_table, index)
     B, width = table.shape
-    seq_len = _i32(seq_len, dev, "seq_len", B)
+    seq_len = _i32(seq_len, index, "seq_len", B)
     p_cu = p_keep = p_acc = p_pos = p_freq = p_q = p_qo = qs = None
     w = n_freq = Hq = 0
     if cu_q is not None:
-        cu_q = _i32(cu_q, dev, "cu_q", B + 1)
+        cu_q = _i32(cu_q, index, "cu_q", B + 1)
         p_cu = cu_q.data_ptr()
     if keep is not None or accepted is not None:
         if keep is None or accepted is None or cu_q is None:
             raise ValueError("append_paged: keep, accepted and cu_q go together")
-        keep = _i32(keep, dev, "keep")
-        accepted = _i32(accepted, dev, "accepted", B)
+        keep = _i32(keep, index, "keep")
+        accepted = _i32(accepted, index, "accepted", B)
         if keep.dim() != 2 or keep.shape[0] != B:
             raise ValueError("append_paged: keep must be [B, w]")
         w, p_keep, p_acc = keep.shape[1], keep.data_ptr(), accepted.data_ptr()
     if inv_freq is not None:
-        if inv_freq.dtype is not torch.float32 or inv_freq.device != dev or not inv_freq.is_contiguous():
-            inv_freq = inv_freq.to(device=dev, dtype=torch.float32).contiguous()
+        if inv_freq.dtype is not torch.float32 or inv_freq.get_device() != index or not inv_freq.is_contiguous():
+            inv_freq = inv_freq.to(device=index, dtype=torch.float32).contiguous()
         n_freq = inv_freq.numel()
         p_freq = inv_freq.data_ptr()
         if 2 * n_freq > D:
             raise ValueError("append_paged: inv_freq has more pairs than half a head")
     if positions is not None:
-        positions = _i32(positions, dev, "positions", total)
+        positions = _i32(positions, index, "positions", total)
         p_pos = positions.data_ptr()
     if q is not None:
         if n > 1 or keep is not None or n_freq == 0:
             raise ValueError("append_paged: q goes with one layer and inv_freq, and not with keep")
         s, shape_q = q.stride(), q.shape
-        if len(shape_q) != 3 or shape_q[0] != total or shape_q[2] != D or q.dtype is not dtype or q.device != dev or s[2] != 1:
+        if len(shape_q) != 3 or shape_q[0] != total or shape_q[2] != D or q.dtype is not dtype or q.get_device() != index or s[2] != 1:
             raise ValueError("append_paged: q must be [total, H_q, D] of the pages' dtype and device, dim stride 1")
         if q_out is None:
             q_out = torch.empty_like(q)
         o = q_out.stride()
-        if q_out.shape != shape_q or q_out.dtype is not dtype or q_out.device != dev or o[2] != 1:
+        if q_out.shape != shape_q or q_out.dtype is not dtype or q_out.get_device() != index or o[2] != 1:
             raise ValueError("append_paged: q_out must be like q, dim stride 1")
         Hq, p_q, p_qo, qs = shape_q[1], q.data_ptr(), q_out.data_ptr(), _I4(s[0], s[1], o[0], o[1])
     elif q_out is not None:
         raise ValueError("append_paged: q_out without q")
     ptrs = struct.Struct(f"{2 * n}P").pack if n > 1 else _P2
-    _launch(dev.index, _lib.lib().cast_paged_append, "cast_paged_append", n, ptrs(*pages), ptrs(*new), _DTYPES[dtype], H,
+    _launch(index, _lib.lib().cast_paged_append, "cast_paged_append", n, ptrs(*pages), ptrs(*new), _DTYPES[dtype], H,
             D, num_pages, ps, _I6(sp[0], sp[1], sp[2], sp[0], sp[1], sp[2]), total, _I4(sk[0], sk[1], sv[0], sv[1]),
             table.data_ptr(), table.stride(0), width, seq_len.data_ptr(), B, p_cu, p_keep, w, p_acc, p_pos, p_freq,
             n_freq, interleaved, rope_scale, p_q, p_qo, Hq, qs)
@@ -237,36 +237,36 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     float32, bfloat16 or float16, D 64 or 128, any H_q / H_kv. The key ranges of all sequences are split evenly
     over the GPU, whatever their lengths; results do not depend on timing.
     """
-    (num_pages, H_kv, ps, D), sp, dtype, dev = _pages(k_pages, v_pages, "decode_attention_paged")
+    (num_pages, H_kv, ps, D), sp, dtype, index = _pages(k_pages, v_pages, "decode_attention_paged")
     shape = q.shape
-    if len(shape) != 3 or shape[2] != D or q.dtype is not dtype or q.device != dev:
+    if len(shape) != 3 or shape[2] != D or q.dtype is not dtype or q.get_device() != index:
         raise ValueError("decode_attention_paged: q must be [B, H_q, D] of the pages' dtype and device")
     B, H_q, _ = shape
     assert H_q % H_kv == 0
-    table = _table(page_table, dev)
+    table = _table(page_table, index)
     rows, width = table.shape
     if rows != B:
         raise ValueError("decode_attention_paged: page_table must have one row per sequence")
-    seq_len = _i32(seq_len, dev, "seq_len", B)
+    seq_len = _i32(seq_len, index, "seq_len", B)
     if window < 0 or not (softcap == 0.0 or 1e-6 <= softcap <= 1e30):
         raise ValueError("decode_attention_paged: window must not be negative, softcap 0 or 1e-6 to 1e30")
     q, sq, p_q = _input(q)
-    out, so, p_out = _output(out, q, shape, dtype, dev)
+    out, so, p_out = _output(out, q, shape, dtype, index)
     p_slopes = p_lse = None
     if alibi_slopes is not None:
-        if alibi_slopes.dtype is not torch.float32 or alibi_slopes.device != dev or not alibi_slopes.is_contiguous():
-            alibi_slopes = alibi_slopes.to(device=dev, dtype=torch.float32).contiguous()
+        if alibi_slopes.dtype is not torch.float32 or alibi_slopes.get_device() != index or not alibi_slopes.is_contiguous():
+            alibi_slopes = alibi_slopes.to(device=index, dtype=torch.float32).contiguous()
         if alibi_slopes.shape != (H_q,):
             raise ValueError("alibi_slopes must be [H_q]")
         p_slopes = alibi_slopes.data_ptr()
     if lse is not None:
-        if lse.shape != (B, H_q) or lse.dtype is not torch.float32 or lse.device != dev or not lse.is_contiguous():
+        if lse.shape != (B, H_q) or lse.dtype is not torch.float32 or lse.get_device() != index or not lse.is_contiguous():
             raise ValueError("lse must be a contiguous float32 [B, H_q]")
         p_lse = lse.data_ptr()
     code = _DTYPES[dtype]
-    n = _decode_bytes(dev.index, code, B, H_q, H_kv, D)
-    workspace = _workspace(workspace, n, dev)
-    _launch(dev.index, _lib.lib().cast_paged_decode_attn, "cast_paged_decode_attn", p_q, k_pages.data_ptr(),
+    n = _decode_bytes(index, code, B, H_q, H_kv, D)
+    workspace = _workspace(workspace, n, index)
+    _launch(index, _lib.lib().cast_paged_decode_attn, "cast_paged_decode_attn", p_q, k_pages.data_ptr(),
             v_pages.data_ptr(), p_out, p_lse, code, _I7(sq[0], sq[1], sp[0], sp[1], sp[2], so[0], so[1]),
             table.data_ptr(), table.stride(0), width, seq_len.data_ptr(), B, H_q, H_kv, D, num_pages, ps,
             0.0 if sm_scale is None else sm_scale, softcap, window, p_slopes,
@@ -285,20 +285,20 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
     pages, whatever their size; float32 on the exact CUDA-core kernel. D 64 or 128.
     max_pack / max_prefix bound pack_len and prefix_len; given, the call reads nothing back to the host.
     """
-    (num_pages, H_kv, ps, D), sp, dtype, dev = _pages(k_pages, v_pages, "varlen_tree_attention_paged")
+    (num_pages, H_kv, ps, D), sp, dtype, index = _pages(k_pages, v_pages, "varlen_tree_attention_paged")
     shape = q.shape
     total_q, H_q, _ = shape
     assert H_q % H_kv == 0
     if shape[2] != D or k_pack.shape != (total_q, H_kv, D) or v_pack.shape != k_pack.shape or q.dtype is not dtype \
-            or k_pack.dtype is not dtype or v_pack.dtype is not dtype or q.device != dev or k_pack.device != dev \
-            or v_pack.device != dev:
+            or k_pack.dtype is not dtype or v_pack.dtype is not dtype or q.get_device() != index or k_pack.get_device() != index \
+            or v_pack.get_device() != index:
         raise ValueError("q must be [total_q, H_q, D] and the packs [total_q, H_kv, D], of the pages' dtype and device")
     if (ancestor_mask is None) == (parent is None):
         raise ValueError("pass exactly one of ancestor_mask and parent")
-    table = _table(page_table, dev)
+    table = _table(page_table, index)
     B, width = table.shape
-    cu_q = _i32(cu_q, dev, "cu_q", B + 1)
-    prefix_len, pack_len = _i32(prefix_len, dev, "prefix_len", B), _i32(pack_len, dev, "pack_len", B)
+    cu_q = _i32(cu_q, index, "cu_q", B + 1)
+    prefix_len, pack_len = _i32(prefix_len, index, "prefix_len", B), _i32(pack_len, index, "pack_len", B)
     if max_pack is None:
         max_pack = int(pack_len.max().item()) if B > 0 else 0
     if max_prefix is None:
@@ -306,23 +306,23 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
     q, sq, p_q = _input(q)
     k_pack, sk, p_k = _input(k_pack)
     v_pack, sv, p_v = _input(v_pack)
-    out, so, p_out = _output(out, q, shape, dtype, dev)
+    out, so, p_out = _output(out, q, shape, dtype, index)
     anc_ptr, wpr, par_ptr = None, 0, None
     if ancestor_mask is not None:
         anc = ancestor_mask
-        if not isinstance(anc, torch.Tensor) or anc.dtype is not torch.int64 or anc.device != dev or not anc.is_contiguous():
-            anc = torch.as_tensor(anc, device=dev).to(torch.int64).contiguous()
+        if not isinstance(anc, torch.Tensor) or anc.dtype is not torch.int64 or anc.get_device() != index or not anc.is_contiguous():
+            anc = torch.as_tensor(anc, device=torch.device("cuda", index)).to(torch.int64).contiguous()
         wpr = anc.numel() // max(total_q, 1)
         if anc.numel() != wpr * total_q:
             raise ValueError("ancestor_mask must be [total_q] or [total_q, words]")
         anc_ptr = anc.data_ptr()
     else:
-        parent = _i32(parent, dev, "parent", total_q)
+        parent = _i32(parent, index, "parent", total_q)
         par_ptr = parent.data_ptr()
     code = _DTYPES[dtype]
-    n = _tree_bytes(dev.index, code, B, total_q, H_q, H_kv, D, max_pack, max_prefix)
-    workspace = _workspace(workspace, n, dev)
-    _launch(dev.index, _lib.lib().cast_tree_attn_paged_fwd, "cast_tree_attn_paged_fwd", p_q, k_pages.data_ptr(),
+    n = _tree_bytes(index, code, B, total_q, H_q, H_kv, D, max_pack, max_prefix)
+    workspace = _workspace(workspace, n, index)
+    _launch(index, _lib.lib().cast_tree_attn_paged_fwd, "cast_tree_attn_paged_fwd", p_q, k_pages.data_ptr(),
             v_pages.data_ptr(), p_k, p_v, p_out, code,
             _I11(sq[0], sq[1], sp[0], sp[1], sp[2], sk[0], sk[1], sv[0], sv[1], so[0], so[1]), table.data_ptr(),
             table.stride(0), width, cu_q.data_ptr(), prefix_len.data_ptr(), pack_len.data_ptr(), anc_ptr, wpr, par_ptr,
