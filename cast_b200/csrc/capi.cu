@@ -1147,22 +1147,22 @@ bool page_strides_ok(const int64_t* st, int elem_bytes) {
 template <typename T>
 cudaError_t launch_append(papp::Args& a, const papp::Layers& ly, bool vec, int nl, int64_t rows, int sms, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
-  const int v = vec ? V : 1;
-  if (a.interleaved && vec) {
-    a.X = a.D / v;
-    a.np = 0;
+  if (vec) {
+    a.np = a.interleaved ? 0 : a.h / V;
+    a.X = a.D / (2 * V);
   } else {
-    a.np = a.h / v;
-    a.X = a.np + (a.D - 2 * a.h) / v;
+    a.np = a.h;
+    a.X = a.D - a.h;
   }
-  const uint64_t heads = (uint64_t)a.H_q + 2 * a.H_kv;
+  const int heads = a.H_q + 2 * a.H_kv;
   a.heads_inv = (uint32_t)((0x100000000ull + heads - 1) / heads);
-  int64_t blocks;
+  // rows that a CTA's threads load at once
+  a.tok = std::min(papp::MAX_TOK, std::max(1, papp::NT / a.X * papp::UNROLL / heads));
+  int64_t blocks = a.B;
   if (a.keep) {
-    a.tok = papp::MAX_TOK;
-    blocks = a.B;
+    a.tok = std::min(a.tok, 4);      // accepted paths are short
   } else {
-    a.tok = rows * nl >= (int64_t)papp::MAX_TOK * 8 * sms ? papp::MAX_TOK : 1;
+    while (a.tok > 1 && rows * nl < (int64_t)a.tok * 8 * sms) --a.tok;
     blocks = (rows + a.tok - 1) / a.tok;
   }
   const dim3 grid((unsigned)blocks, (unsigned)nl);
@@ -1273,8 +1273,8 @@ int cast_paged_append(int n_layers, void* const* pages_kv, const void* const* ne
   a.table = page_table; a.seq_len = seq_len; a.cu_q = cu_q; a.keep = keep; a.accepted = accepted;
   a.positions = positions; a.keep_stride = keep_stride; a.inv_freq = inv_freq;
   a.q = q; a.q_out = q_out;
-  // 16-byte pieces where every head and every half of a rotated head starts on one
-  bool vec = D % v == 0 && (interleaved ? 2 * n_freq : n_freq) % v == 0;
+  // 16-byte pieces, two to a thread, where every head and every half of a rotated head starts on one
+  bool vec = D % (2 * v) == 0 && (interleaved ? 2 * n_freq : n_freq) % v == 0;
   for (int i = 0; i < 6; ++i) vec = vec && page_strides[i] % v == 0;
   for (int i = 0; i < 4; ++i) vec = vec && new_strides[i] % v == 0 && (!q || q_strides[i] % v == 0);
   vec = vec && (!q || (aligned(q, 16) && aligned(q_out, 16)));

@@ -10,12 +10,12 @@
 // are 32-bit, and each result is rounded once to the cache's type.
 //
 // Bound: memory traffic for prompts (2 bytes moved per byte of k, v and q), the latency of the chain
-// length -> table entry -> store for a few rows. One CTA takes `tok` consecutive rows (2 when that still
-// gives every SM several CTAs, else 1) and all their heads, so an angle is computed once per row and
-// shared by H_q + H_kv heads through shared memory. Thread (x, y): x = 16-byte pieces of a head, y steps
-// over (row, head); a piece of the first half travels with its partner of the second half, so both
-// results come from one thread's registers. The first loads are issued before the row's sequence, page
-// and angles are known.
+// length -> table entry -> store for a few rows. One CTA takes `tok` consecutive rows (what its threads
+// load at once, fewer where that leaves SMs without eight CTAs) and all their heads, so an angle is
+// computed once per row and shared by H_q + H_kv heads through shared memory. Thread (x, y): x = two
+// 16-byte pieces of a head, y steps over (row, head); a piece of the first half travels with its partner
+// of the second half, so both results come from one thread's registers. The first loads are issued before
+// the row's sequence, page and angles are known.
 #pragma once
 
 #include "common.cuh"
@@ -24,7 +24,7 @@ namespace cast {
 namespace papp {
 
 constexpr int NT = 256;
-constexpr int MAX_TOK = 2;      // rows per CTA
+constexpr int MAX_TOK = 8;      // rows per CTA
 constexpr int MAX_D = 256;
 constexpr int MAX_HEADS = 4096;
 constexpr int MAXL = 64;        // layers per launch
@@ -38,7 +38,7 @@ struct Layers {
 struct Args {
   int H_kv, H_q, D, h;                 // h = rotated pairs per head
   int interleaved, tok;
-  int X, np;                           // pieces per head and thread column count; paired pieces
+  int X, np;                           // threads per head; those that hold the two pieces of a rotated pair
   uint32_t heads_inv;                  // ceil(2^32 / (H_q + 2 H_kv)): i / heads for i < 2^16
   float rope_scale;
   int num_pages, page_size, max_pages, B;
@@ -134,6 +134,29 @@ __device__ __forceinline__ void turn(Piece<T, VEC>& a, Piece<T, VEC>& b, const f
   }
 }
 
+// The pairs (a[2e], a[2e + 1]) turned by (c[e], s[e]).
+template <typename T, int VEC>
+__device__ __forceinline__ void turn_within(Piece<T, VEC>& a, const float* c, const float* s) {
+  if constexpr (sizeof(T) == 2 && VEC == 8) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2* pa = reinterpret_cast<T2*>(a.x);
+    const float4 c4 = *reinterpret_cast<const float4*>(c), s4 = *reinterpret_cast<const float4*>(s);
+    const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 u = pair_to_f(pa[e]);
+      pair_from_f(pa[e], u.x * cc[e] - u.y * ss[e], u.y * cc[e] + u.x * ss[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e + 1 < VEC; e += 2) {
+      const float u = Elem<T>::to_f(a.x[e]), v = Elem<T>::to_f(a.x[e + 1]);
+      a.x[e] = Elem<T>::from_f(u * c[e / 2] - v * s[e / 2]);
+      a.x[e + 1] = Elem<T>::from_f(v * c[e / 2] + u * s[e / 2]);
+    }
+  }
+}
+
 struct RowMeta {
   int64_t row;      // source row, -1: nothing to do
   int64_t dk, dv;   // element offset of the destination row (head 0) in the K / V pages
@@ -154,14 +177,19 @@ __global__ void __launch_bounds__(NT, 4) append_kernel(const Args a, const __gri
   T* qo = static_cast<T*>(a.q_out);
   const int X = a.X, Y = NT / X;           // threads beyond X * Y have no items
   const int x = tid % X, y = tid / X;
-  const bool half_pair = x < a.np;           // a second piece belongs to this one
-  const bool scalar_pairs = a.interleaved && VEC == 1;
-  // offsets inside a rotated head, and inside a value head
-  int off_a, off_b;
-  if (a.interleaved && VEC > 1) { off_a = x * VEC; off_b = 0; }
-  else if (scalar_pairs) { off_a = half_pair ? 2 * x : 2 * a.np + (x - a.np); off_b = 2 * x + 1; }
-  else { off_a = half_pair ? x * VEC : 2 * a.h + (x - a.np) * VEC; off_b = a.h + x * VEC; }
+  // A thread's pieces, at off_a and off_b of a rotated head and voff_a and voff_b of a value head: two
+  // halves of a pair (x < np), or two pieces of those that pass through or hold their pairs within
+  // themselves (`inner`). Single elements (VEC = 1) that pass through come one to a thread.
+  const bool paired = x < a.np, two = VEC > 1 || paired, inner = VEC > 1 && a.interleaved;
   const int voff_a = x * VEC, voff_b = (X + x) * VEC;
+  int off_a = voff_a, off_b = voff_b;
+  if (VEC == 1 && a.interleaved) {
+    off_a = paired ? 2 * x : a.np + x;
+    off_b = 2 * x + 1;
+  } else if (!inner) {
+    off_a = paired ? x * VEC : 2 * a.h + (x - a.np) * VEC;
+    off_b = paired ? a.h + x * VEC : a.h + (X + x - a.np) * VEC;
+  }
   const int heads = a.H_q + 2 * a.H_kv;      // H_q = 0 without queries
   // accept mode: one CTA per sequence walks its accepted rows; else one CTA per `tok` rows
   const bool accept = a.keep != nullptr;
@@ -197,7 +225,7 @@ __global__ void __launch_bounds__(NT, 4) append_kernel(const Args a, const __gri
       else if (!is_v) src = sk + row * a.sk_t + (hd - a.H_q) * a.sk_h;
       else src = sv + row * a.sv_t + (hd - a.H_q - a.H_kv) * a.sv_h;
       pa[u] = load_piece<T, VEC>(src + (is_v ? voff_a : off_a));
-      if (half_pair) pb[u] = load_piece<T, VEC>(src + (is_v ? voff_b : off_b));
+      if (two) pb[u] = load_piece<T, VEC>(src + (is_v ? voff_b : off_b));
     }
   };
   auto store = [&](int i0) {
@@ -214,23 +242,15 @@ __global__ void __launch_bounds__(NT, 4) append_kernel(const Args a, const __gri
       else if (!is_v) dst = dk + m.dk + (hd - a.H_q) * a.pk_h;
       else dst = dv + m.dv + (hd - a.H_q - a.H_kv) * a.pv_h;
       if (!is_v) {
-        if (a.interleaved && VEC > 1) {
-          if (x * VEC < 2 * a.h) {
-            const float* c = cs[k] + x * (VEC / 2);
-            const float* s = sn[k] + x * (VEC / 2);
-#pragma unroll
-            for (int e = 0; e + 1 < VEC; e += 2) {
-              const float u0 = Elem<T>::to_f(pa[u].x[e]), u1 = Elem<T>::to_f(pa[u].x[e + 1]);
-              pa[u].x[e] = Elem<T>::from_f(u0 * c[e / 2] - u1 * s[e / 2]);
-              pa[u].x[e + 1] = Elem<T>::from_f(u1 * c[e / 2] + u0 * s[e / 2]);
-            }
-          }
-        } else if (half_pair) {
+        if (inner) {
+          if (off_a < 2 * a.h) turn_within<T, VEC>(pa[u], cs[k] + off_a / 2, sn[k] + off_a / 2);
+          if (off_b < 2 * a.h) turn_within<T, VEC>(pb[u], cs[k] + off_b / 2, sn[k] + off_b / 2);
+        } else if (paired) {
           turn<T, VEC>(pa[u], pb[u], cs[k] + x * VEC, sn[k] + x * VEC);
         }
       }
       store_piece<T, VEC>(dst + (is_v ? voff_a : off_a), pa[u]);
-      if (half_pair) store_piece<T, VEC>(dst + (is_v ? voff_b : off_b), pb[u]);
+      if (two) store_piece<T, VEC>(dst + (is_v ? voff_b : off_b), pb[u]);
     }
   };
   for (int rd = 0; rd < rounds; ++rd) {
