@@ -6,7 +6,7 @@
 // Bound: one read of the visible keys and values from HBM (4 flops per byte and query head of a KV head).
 //
 // Split: every warp is a worker of its own. The visible keys of all (sequence, KV head, tile of query
-// heads) units, in steps of 16 keys (8 in 32 bits at D = 128), form one list of T steps, cut into n even groups of steps whatever
+// heads) units, in steps of 4 KB of keys (16 keys of 128 16-bit values), form one list of T steps, cut into n even groups of steps whatever
 // units they fall into, so ragged lengths load every warp alike and no host read of the lengths is needed.
 // A long group is cut once more, into a head and NS short tails: the CTAs of the heads come first in the
 // grid and fill the GPU, those of the tails start as slots get free. Some SMs read memory a tenth slower
@@ -37,7 +37,7 @@ constexpr int TAIL = 12;         // each 1 / TAIL of it,
 constexpr int MIN_TAIL = 8;      // and of at least this many steps (tails of 4 cost a sequence of 131072 keys a tenth)
 
 // Keys per step, and ring stages per worker: eight workers per SM (two CTAs) hold 192 KB.
-template <typename T, int D> __host__ __device__ constexpr int step_keys() { return sizeof(T) == 4 && D == 128 ? 8 : 16; }
+template <typename T, int D> __host__ __device__ constexpr int step_keys() { return 4096 / (D * (int)sizeof(T)); }
 template <typename T, int D> __host__ __device__ constexpr int stage_bytes() { return 2 * step_keys<T, D>() * D * (int)sizeof(T); }
 template <typename T, int D> __host__ __device__ constexpr int stages() { return 24 * 1024 / stage_bytes<T, D>(); }
 constexpr int CTAS_PER_SM = 2;
@@ -409,6 +409,7 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int KS = step_keys<T, D>(), NST = stages<T, D>(), SB = stage_bytes<T, D>(), ROW = D * 2;
+  constexpr int SUB = KS / 16;         // 16-key MMA rows per step
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const Work wk = plan_steps<KS>(p);
@@ -478,51 +479,63 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
     take = take + SB == ring + NST * SB ? ring : take + SB;
     issue();                           // into the stage that the previous step left
 
-    constexpr int NC = NH == 1 ? 2 : 1;      // one tile of heads: two chains of dependent MMAs
-    float s[NH][4], s2[NH][4];
+    constexpr int NC = NH * SUB == 1 ? 2 : 1;      // one tile of heads and keys: two chains of dependent MMAs
+    float s[SUB][NH][4], s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int a = 0; a < NH; ++a)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[a][i] = s2[a][i] = 0.f;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      uint32_t ka[4];
-      ldsm4(st + koff + ((kx ^ (2 * k)) * 16), ka);
-#pragma unroll
-      for (int a = 0; a < NH; ++a) mma16816<T>((k % NC) ? s2[a] : s[a], ka, qf[a][k][0], qf[a][k][1]);
-    }
-    if (NC == 2)
+    for (int e = 0; e < SUB; ++e)
 #pragma unroll
       for (int a = 0; a < NH; ++a)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[a][i] += s2[a][i];
+        for (int i = 0; i < 4; ++i) s[e][a][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int e = 0; e < SUB; ++e) {
+        uint32_t ka[4];
+        ldsm4(st + koff + e * 16 * ROW + ((kx ^ (2 * k)) * 16), ka);
+#pragma unroll
+        for (int a = 0; a < NH; ++a) mma16816<T>((k % NC) ? s2 : s[e][a], ka, qf[a][k][0], qf[a][k][1]);
+      }
+    if (NC == 2)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[0][0][i] += s2[i];
     const int n0 = cc.s * KS + g;
     if (p.modified) {
 #pragma unroll
-      for (int a = 0; a < NH; ++a)
+      for (int e = 0; e < SUB; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[a][i] = modified_score<false>(p, s[a][i] * p.scale, n0 + (i >> 1) * 8, cc.z, slope[a][i & 1]);
+        for (int a = 0; a < NH; ++a)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[e][a][i] = modified_score<false>(p, s[e][a][i] * p.scale, n0 + e * 16 + (i >> 1) * 8, cc.z, slope[a][i & 1]);
     } else {
 #pragma unroll
-      for (int a = 0; a < NH; ++a)
+      for (int e = 0; e < SUB; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[a][i] *= c;
+        for (int a = 0; a < NH; ++a)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[e][a][i] *= c;
     }
     if (n0 - g < cc.z.lo || n0 - g + KS > cc.z.len) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (n0 + i * 8 < cc.z.lo || n0 + i * 8 >= cc.z.len)
+      for (int e = 0; e < SUB; ++e)
 #pragma unroll
-          for (int a = 0; a < NH; ++a) s[a][2 * i] = s[a][2 * i + 1] = -INFINITY;
+        for (int i = 0; i < 2; ++i) {
+          const int n = n0 + e * 16 + i * 8;
+          if (n < cc.z.lo || n >= cc.z.len)
+#pragma unroll
+            for (int a = 0; a < NH; ++a) s[e][a][2 * i] = s[e][a][2 * i + 1] = -INFINITY;
+        }
     }
-    uint32_t ph[NH][2], pl_[NH][2];
+    uint32_t ph[SUB][NH][2], pl_[SUB][NH][2];
 #pragma unroll
     for (int a = 0; a < NH; ++a) {
       float al[2], mu[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float mx = fmaxf(s[a][i], s[a][2 + i]);
+        float mx = fmaxf(s[0][a][i], s[0][a][2 + i]);
+#pragma unroll
+        for (int e = 1; e < SUB; ++e) mx = fmaxf(mx, fmaxf(s[e][a][i], s[e][a][2 + i]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -541,25 +554,29 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float p0 = ex2(s[a][2 * i] - mu[0]), p1 = ex2(s[a][2 * i + 1] - mu[1]);
-        l[a][0] += p0;
-        l[a][1] += p1;
-        split2<T>(p0, p1, ph[a][i], pl_[a][i]);
-        ph[a][i] = transpose8(ph[a][i]);
-        pl_[a][i] = transpose8(pl_[a][i]);
-      }
+      for (int e = 0; e < SUB; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float p0 = ex2(s[e][a][2 * i] - mu[0]), p1 = ex2(s[e][a][2 * i + 1] - mu[1]);
+          l[a][0] += p0;
+          l[a][1] += p1;
+          split2<T>(p0, p1, ph[e][a][i], pl_[e][a][i]);
+          ph[e][a][i] = transpose8(ph[e][a][i]);
+          pl_[e][a][i] = transpose8(pl_[e][a][i]);
+        }
     }
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      uint32_t va[4];
-      ldsm4t(st + voff + ((vx ^ (2 * j)) * 16), va);
+    for (int e = 0; e < SUB; ++e)
 #pragma unroll
-      for (int a = 0; a < NH; ++a) {
-        mma16816<T>(o[a][j], va, ph[a][0], ph[a][1]);
-        mma16816<T>(o[a][j], va, pl_[a][0], pl_[a][1]);
+      for (int j = 0; j < D / 16; ++j) {
+        uint32_t va[4];
+        ldsm4t(st + voff + e * 16 * ROW + ((vx ^ (2 * j)) * 16), va);
+#pragma unroll
+        for (int a = 0; a < NH; ++a) {
+          mma16816<T>(o[a][j], va, ph[e][a][0], ph[e][a][1]);
+          mma16816<T>(o[a][j], va, pl_[e][a][0], pl_[e][a][1]);
+        }
       }
-    }
     const bool unit_end = cc.s + 1 == cc.z.s1;
     if (unit_end || left == 1) {
       const bool direct = whole && unit_end;
@@ -600,7 +617,7 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
 }
 
 // ---------------------------------------------------------------------------------------- 32-bit type
-// GT query heads of one KV head. Scores: lane = key (lane % KS) and part of the head dim (lane / KS);
+// GT query heads of one KV head. Scores: lane = key (lane % KS) and every (32 / KS)-th 16-byte piece of it;
 // outputs: lane = D / 32 dims, over the step's keys.
 template <int D, int GT>
 __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
@@ -671,7 +688,7 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
     for (int a = 0; a < GT; ++a) s[a] = 0.f;
 #pragma unroll 4
     for (int i = 0; i < D / 4 / PARTS; ++i) {
-      const int ch = part * (D / 4 / PARTS) + i;
+      const int ch = i * PARTS + part;
       const float4 x = *reinterpret_cast<const float4*>(st + key * (D * 4) + ((ch ^ (key & 7)) * 16));
 #pragma unroll
       for (int a = 0; a < GT; ++a) {
