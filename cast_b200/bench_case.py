@@ -217,8 +217,10 @@ def vs_triton(args, dev):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--what", choices=["attn", "attn_store", "topk", "tree", "walk", "select", "append", "vs_triton"],
+    ap.add_argument("--what", choices=["attn", "attn_store", "topk", "tree", "walk", "select", "append",
+                                       "attn_paged", "decode_paged", "append_paged", "vs_triton"],
                     default="attn")
+    ap.add_argument("--page", type=int, default=64, help="attn_paged, decode_paged, append_paged: rows per page")
     ap.add_argument("--width", type=int, default=32, help="vs_triton on configuration 5: tree width N (<= 63)")
     ap.add_argument("--config", type=int, default=3)
     ap.add_argument("--batch", type=int, default=32)
@@ -264,6 +266,28 @@ def main():
         args_store = (q, k_store, v_store, k_pack.transpose(0, 1), v_pack.transpose(0, 1), t(lay["cu_q"]),
                       t(lay["prefix_len"]), t(lay["pack_len"]), None)
 
+    if args.what in ("attn_paged", "decode_paged", "append_paged"):
+        # the configuration's prefixes in pages, in a random order, with room for one more row; append_paged
+        # appends a token to each sequence (keys and queries rotated), decode_paged attends over prefix + token
+        ps = args.page
+        width = (max(w.S) + ps) // ps
+        k_pages = torch.zeros((w.B * width, w.H_kv, ps, w.D), dtype=k.dtype, device=dev)
+        v_pages = torch.zeros_like(k_pages)
+        table = torch.randperm(w.B * width, generator=torch.Generator().manual_seed(7)).int().view(w.B, width).to(dev)
+        none = torch.zeros(w.B, dtype=torch.int32, device=dev)
+        length = t(lay["prefix_len"])
+        cast_b200.append_paged(k_pages, v_pages, table, none, k, v, t(lay["cu_kv"]), keep=torch.arange(
+            max(w.S), dtype=torch.int32, device=dev).repeat(w.B, 1), accepted=length)
+        rows = torch.tensor([int(lay["cu_kv"][b]) + w.S[b] for b in range(w.B)], device=dev)
+        q_row = torch.tensor([int(lay["cu_q"][b]) for b in range(w.B)], device=dev)
+        q1, k1, v1 = q[q_row].contiguous(), k[rows].contiguous(), v[rows].contiguous()
+        pack_rows = torch.cat([torch.arange(int(lay["cu_kv"][b]) + w.S[b], int(lay["cu_kv"][b + 1])) for b in range(w.B)])
+        k_pk, v_pk = k[pack_rows.to(dev)].contiguous(), v[pack_rows.to(dev)].contiguous()
+        inv_freq = (10000.0 ** (-torch.arange(0, w.D, 2, dtype=torch.float64) / w.D)).float().to(dev)
+        q1_out, out1, longer = torch.empty_like(q1), torch.empty_like(q1), length + 1
+        ws1 = torch.empty(cast_b200.decode_workspace_size(k.dtype, w.B, w.H_q, w.H_kv, w.D), dtype=torch.uint8, device=dev)
+        del k, v
+
     if args.what in ("walk", "append"):
         gen = torch.Generator(device=dev).manual_seed(7)
         tl = torch.empty((lay["total_q"], w.V), dtype=torch.bfloat16, device=dev)
@@ -294,6 +318,8 @@ def main():
     if args.what == "select":
         sel_src = cast_b200.build_trees(idx, lp, 48, 8, max_budget=48)
 
+    t_pack = t(lay["pack_len"])
+
     def once():
         if args.what == "attn":
             cast_b200.varlen_tree_attention(*args_attn, parent=trees.pack_parent, max_pack=lay["max_pack"],
@@ -301,6 +327,14 @@ def main():
         elif args.what == "attn_store":
             cast_b200.varlen_tree_attention_store(*args_store, parent=trees.pack_parent, max_pack=lay["max_pack"],
                                                   max_prefix=max(w.S), out=out)
+        elif args.what == "attn_paged":
+            cast_b200.varlen_tree_attention_paged(q, k_pages, v_pages, table, k_pk, v_pk, cu_q, length, t_pack, None,
+                                                  parent=trees.pack_parent, max_pack=lay["max_pack"],
+                                                  max_prefix=max(w.S), out=out)
+        elif args.what == "decode_paged":
+            cast_b200.decode_attention_paged(q1, k_pages, v_pages, table, longer, out=out1, workspace=ws1)
+        elif args.what == "append_paged":
+            cast_b200.append_paged(k_pages, v_pages, table, length, k1, v1, inv_freq=inv_freq, q=q1, q_out=q1_out)
         elif args.what == "topk":
             cast_b200.block_topk_device(logits, 8, idx, lp)
         elif args.what == "walk":
@@ -343,7 +377,9 @@ def main():
         if _lib.device_error() != 0:
             raise RuntimeError("device error")
         rec["us_per_launch_graph"] = round(ev[0].elapsed_time(ev[1]) * 1e3 / args.iters, 1)
-    if args.what in ("attn", "attn_store"):
+    if args.what == "decode_paged":
+        rec["gbs"] = round(sum(n + 1 for n in w.S) * w.H_kv * w.D * 2 * q.element_size() / rec["us_per_launch"] * 1e-3, 1)
+    if args.what in ("attn", "attn_store", "attn_paged"):
         # achieved work against the measured peaks (MEASURED_PEAKS.json beside the package, else the
         # earlier measurement on this pool); a kernel timed alone is compared with the burst figures
         import pathlib

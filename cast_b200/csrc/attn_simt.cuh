@@ -406,8 +406,8 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const AttnParams p) {
     float4 x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int z = min(z0 + k, nsplit - 1);
-      const int64_t slot = slot0 + z * slots;
+      if (z0 + k >= nsplit) break;
+      const int64_t slot = slot0 + (z0 + k) * slots;
       ml[k] = *reinterpret_cast<const float2*>(p.ws_ml + slot * 2);
       x[k] = has ? *reinterpret_cast<const float4*>(p.ws_o + slot * p.D + c) : make_float4(0.f, 0.f, 0.f, 0.f);
     }

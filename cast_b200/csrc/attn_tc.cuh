@@ -135,11 +135,17 @@ __device__ __forceinline__ int ranked_sequence(const AttnParams& p, int rank, in
 // page (the 128-byte swizzle goes by the shared-memory address, so boxes of fewer than 8 rows land as
 // one of 128 would put them). The producer warp's lanes issue them side by side, each from a table
 // entry that it read while the previous tile was under way.
+// kPagedRows: as kPaged for boxes of fewer than 8 rows (page sizes that are no multiple of 8), where the
+// number of copies was the bound (256 per tile and tensor for pages of one row). The producer warps copy
+// the prefix rows with 16-byte asynchronous copies into the swizzled places, two rows an instruction; their
+// completion arrives on the tile's barrier (32 arrivals), and the MMA warp fences the tile for the tensor
+// core before it reads it. 64 packs of 128 over 4000 keys in pages of one row: 2910 us by boxes, 711 by
+// rows (557 with pages of 16; a row's address costs the copying warp two shuffles and an addition).
 // Head groups that do not divide 128 (paged only) take p.bm = 128 / G * G rows of each query tile: the
 // copies leave the last rows of the tile's shared memory as they were, the MMAs compute on them, and
 // nothing is written for them (a row of S, P or O depends on its own row of Q alone). DH = 64 uses the
 // first of a tile's two 64-column panels.
-enum KvLayout { kRagged = 0, kStore = 1, kPaged = 2 };
+enum KvLayout { kRagged = 0, kStore = 1, kPaged = 2, kPagedRows = 3 };
 template <bool BF16, int LAYOUT, int DH = 128>
 __global__ void __launch_bounds__(NT, 1)
 attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -147,8 +153,9 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
                const __grid_constant__ CUtensorMap tmVp) {
   using namespace tc;
   constexpr bool STORE = LAYOUT != kRagged;   // prefix tiles and pack tiles come from different tensors
+  constexpr bool PAGED = LAYOUT >= kPaged, BY_ROWS = LAYOUT == kPagedRows;
   constexpr int D = DH, PANELS = DH / 64;
-  if constexpr (LAYOUT == kPaged) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if constexpr (PAGED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* sAnc = reinterpret_cast<uint64_t*>(smem + SMEM_ANC);
@@ -191,7 +198,7 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
     return;
   }
   const int G = p.G;
-  const int bm = LAYOUT == kPaged ? p.bm : BM;   // rows of a query tile
+  const int bm = PAGED ? p.bm : BM;   // rows of a query tile
   const int rows = G * m.P;
   if (p.tail_only) {   // only the sequence's partial last 256-row block (the CTA-pair launch runs the rest)
     if (rows % (QT * BM) == 0) return;
@@ -241,9 +248,9 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
   if (tid == 0) {
     mbar_init(smem_u32(&bars.q_full), 1);
     for (int s = 0; s < NST; ++s) {
-      mbar_init(smem_u32(&bars.k_full[s]), 1);
+      mbar_init(smem_u32(&bars.k_full[s]), BY_ROWS ? 32 : 1);
       mbar_init(smem_u32(&bars.k_empty[s]), 1);
-      mbar_init(smem_u32(&bars.v_full[s]), 1);
+      mbar_init(smem_u32(&bars.v_full[s]), BY_ROWS ? 32 : 1);
       mbar_init(smem_u32(&bars.v_empty[s]), 1);
     }
     for (int q = 0; q < QT; ++q) {
@@ -285,6 +292,49 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
   };
   int next_page = -1;
   if (LAYOUT == kPaged && (warp == 0 || warp == 2)) next_page = page_at(t_begin * BN + lane / PANELS * p.box);
+  // kPagedRows: the table entries of rows lane, lane + 32, ... of the next prefix tile
+  int row_page[BY_ROWS ? BN / 32 : 1];
+  auto read_pages = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < BN / 32; ++i)
+      if (BY_ROWS) row_page[i % (BY_ROWS ? BN / 32 : 1)] = t < nt_pre ? page_at(t * BN + i * 32 + lane) : -1;
+  };
+  if (BY_ROWS && (warp == 0 || warp == 2)) read_pages(t_begin);
+  auto copy_rows = [&](int t, uint32_t dst) {
+    constexpr int CH = D / 8, RPI = 32 / CH;             // 16-byte pieces of a row, rows an instruction
+    const char* base = static_cast<const char*>(is_k ? p.k_pages : p.v_pages) + (int64_t)h * p.pg_h * 2;
+    const int c = lane % CH, r0 = lane / CH;
+    const uint32_t to = dst + (c / 8) * HALF_BYTES;
+#pragma unroll
+    for (int i = 0; i < BN / 32; ++i) {
+      const int n = t * BN + i * 32 + lane, page = row_page[i % (BY_ROWS ? BN / 32 : 1)];
+      int64_t off = -1;
+      if (n < m.S) {
+        if (page >= 0 && page < p.num_pages) off = ((int64_t)page * p.pg_p + (int64_t)(n % p.page_size) * p.pg_r) * 2;
+        else report(CAST_DEV_BAD_LAYOUT);
+      }
+      const char* row = base + (off >= 0 ? off : 0);
+      const uint32_t at = to + (i * 32 + r0) * 128;
+      if (__all_sync(0xffffffffu, off >= 0)) {
+#pragma unroll
+        for (int k = 0; k < 32 / RPI; ++k) {
+          const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row), k * RPI + r0));
+          const int swz = (((c % 8) ^ r0) ^ (k * RPI % 8)) * 16;      // r0 < RPI <= 4, k RPI a multiple of RPI
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + k * RPI * 128 + swz), "l"(src + c * 16) : "memory");
+        }
+      } else {
+#pragma unroll 4
+        for (int k = 0; k < 32 / RPI; ++k) {
+          const int64_t o = __shfl_sync(0xffffffffu, off, k * RPI + r0);
+          const int swz = (((c % 8) ^ r0) ^ (k * RPI % 8)) * 16;
+          const int size = o >= 0 ? 16 : 0;                // 0: zeros, nothing read
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + k * RPI * 128 + swz),
+                       "l"(base + (o >= 0 ? o : 0) + c * 16), "r"(size) : "memory");
+        }
+      }
+    }
+    read_pages(t + 1);
+  };
   // one 128-key tile (two 64-column halves) into ring slot j % NST
   auto issue_tile = [&](int j) {
     const uint32_t dst = ring + (j % NST) * TILE_BYTES, bar = smem_u32(&full[j % NST]);
@@ -304,7 +354,12 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
         }
         tma_load_4d(dst + lane % PANELS * HALF_BYTES + i * p.box * 128, m_reg, lane % PANELS * 64, n % p.page_size, h, page, bar);
       }
-    } else if (elect_one()) {
+    } else if (BY_ROWS && t < nt_pre) {
+      copy_rows(t, dst);
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+    } else if (!elect_one()) {
+      if (BY_ROWS) mbar_arrive(bar);
+    } else {
       mbar_expect_tx(bar, PANELS * HALF_BYTES);
       for (int hf = 0; hf < PANELS; ++hf) {
         if constexpr (STORE) {
@@ -396,7 +451,9 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
       __syncwarp();
     };
     auto wait_all = [&](uint64_t& bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), parity, abort_flag, p.wait_ns));
+      const bool done = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), parity, abort_flag, p.wait_ns));
+      if (BY_ROWS) fence_proxy_async_smem();   // rows written by asynchronous copies, read by the MMAs
+      return done;
     };
     // Store mode: the last prefix tile also holds store rows past the prefix; their scores
     // are masked, but 0 x (a non-finite stale value) would still poison P V, so those V rows
@@ -629,7 +686,7 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
         }
       };
       if (done) {
-        const bool store = r < rows && (LAYOUT != kPaged || t < bm);
+        const bool store = r < rows && (!PAGED || t < bm);
         const int i = min(r / G, m.P - 1), hq = h * G + r % G;
         const int64_t tq = m.q0 + i;
         if (p.n_split == 1) {

@@ -262,7 +262,7 @@ int launch_tc_maps(AttnParams& p, const TcPlan& pl, int dtype, cudaStream_t st, 
   p.m_tiles = pl.m_blocks;
   p.W = pl.W;
   {
-    const int bm = LAYOUT == tca::kPaged ? p.bm : tca::BM;
+    const int bm = LAYOUT >= tca::kPaged ? p.bm : tca::BM;
     const long long last = ((long long)p.G * p.max_pack) % (tca::QT * bm);
     p.tail_last = (last > 0 && last <= bm) ? 1 : 0;
   }
@@ -277,7 +277,7 @@ int launch_tc_maps(AttnParams& p, const TcPlan& pl, int dtype, cudaStream_t st, 
   }
   if (cudaGetLastError() != cudaSuccess) return CAST_ERR_LAUNCH;
   if (!combine || pl.n_split == 1) return CAST_OK;
-  constexpr bool early = LAYOUT == tca::kPaged;
+  constexpr bool early = LAYOUT >= tca::kPaged;
   return dtype == CAST_BF16 ? launch_combine<__nv_bfloat16>(p, early, st) : launch_combine<__half>(p, early, st);
 }
 
@@ -1464,6 +1464,9 @@ int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_p
       !make_map(&mkp, k_pack, dtype, total_q, H_kv, skp[0], skp[1], 1, tca::BN, D) ||
       !make_map(&mvp, v_pack, dtype, total_q, H_kv, svp[0], svp[1], 1, tca::BN, D))
     return CAST_ERR_LAUNCH;
+  if (p.box < 8)
+    return D == 128 ? launch_tc_maps<tca::kPagedRows, 128>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp)
+                    : launch_tc_maps<tca::kPagedRows, 64>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp);
   return D == 128 ? launch_tc_maps<tca::kPaged, 128>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp)
                   : launch_tc_maps<tca::kPaged, 64>(p, pl, dtype, st, mq, mks, mvs, mkp, mvp);
 }

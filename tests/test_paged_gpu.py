@@ -288,6 +288,13 @@ def test_decode_pages(cuda, dtype, ps, order):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("ps,order", [(1, "nhd"), (5, "hnd"), (8, "hnd"), (40, "nhd")])
+def test_decode_pages_of_small_heads(cuda, dtype, ps, order):
+    # D = 64: steps of 32 keys (16 in 32 bits), which pages of fewer rows cut
+    _run_decode(cuda, 27, [5, 130, 64, 999, 31, 32, 33], 6, 2, 64, ps, TYPES[dtype], order, window=700)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("cap,window,alibi", [(20.0, 0, False), (0.0, 1, False), (0.0, 50, False), (0.0, 0, True),
                                               (30.0, 130, True), (0.0, 5000, False)])
 def test_decode_score_options(cuda, dtype, cap, window, alibi):
@@ -347,6 +354,41 @@ def test_decode_cache_beyond_32_bit_offsets(cuda):
         out, _, e, pv = _attend(q, kk, vv, 1 / math.sqrt(D), 0, None, None)
         _check_attention(tree[i:i + 1], out, e, pv, n + i + 1, torch.bfloat16, _half(torch.bfloat16))
     del k, v
+
+
+def test_decode_tails_of_long_groups(cuda):
+    # 16 sequences of 16000 keys, 8 heads: 128000 steps are 108 to a group, so the groups end in two tails; a table with
+    # no room to spare. Also: the same call twice gives the same bits, and padded rows of the batch (length 0) give 0.
+    lens = [16000] * 15 + [15999, 0]
+    c = Cache(30, lens, 8, 128, 64, torch.bfloat16, cuda, poison=False)
+    g = torch.Generator(device=cuda).manual_seed(31)
+    q = torch.empty((17, 32, 128), dtype=torch.bfloat16, device=cuda).normal_(generator=g)
+    got = cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, c.len)
+    assert torch.equal(got, cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, c.len))
+    assert _lib.device_error() == 0 and (got[16] == 0).all()
+    for b in (0, 3, 7, 11, 15):
+        k, v = c.rows(c.k[0], b, 0, lens[b]), c.rows(c.v[0], b, 0, lens[b])
+        out, _, e, pv = _attend(q[b:b + 1], k, v, 1 / math.sqrt(128), 0, None, None)
+        _check_attention(got[b:b + 1], out, e, pv, lens[b], torch.bfloat16, 2.0 ** -15)
+
+
+def test_decode_two_streams_with_their_own_workspaces(cuda):
+    c = Cache(33, [5000, 700, 9000], 4, 128, 16, torch.float16, cuda, poison=False)
+    g = torch.Generator(device=cuda).manual_seed(34)
+    q = torch.empty((3, 16, 128), dtype=torch.float16, device=cuda).normal_(generator=g)
+    want = cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, c.len)
+    torch.cuda.synchronize()
+    n = cast_b200.decode_workspace_size(torch.float16, 3, 16, 4, 128)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ws = [torch.empty(n, dtype=torch.uint8, device=cuda) for _ in streams]
+    outs = [[torch.empty_like(q) for _ in range(5)] for _ in streams]
+    torch.cuda.synchronize()
+    for i in range(5):
+        for s, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, c.len, out=outs[s][i], workspace=ws[s])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for os in outs for o in os)
 
 
 def test_decode_graph_streams_and_repeats(cuda):
@@ -449,6 +491,33 @@ def test_tree_heads(cuda, dtype, Hq, Hkv, D):
                                                 parent=np.concatenate(parents))
     assert _lib.device_error() == 0
     _check_tree(got, c, q, kp, vp, [_seen(p) for p in parents], cu, S, dt, 0.0 if dtype == "fp32" else _half(dt))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("Hq,Hkv,D,ps", [(3, 1, 64, 1), (10, 2, 128, 5), (8, 2, 64, 12)])
+def test_tree_rows_of_odd_pages(cuda, dtype, Hq, Hkv, D, ps):
+    # pages that are no multiple of 8: rows copied one by one, over several tiles and an unfinished one
+    S, P = [700, 0, 129, 128], [9, 1, 130, 64]
+    dt = TYPES[dtype]
+    c, q, kp, vp, parents, cu = _tree_inputs(cuda, 28, S, P, Hq, Hkv, D, ps, dt)
+    got = cast_b200.varlen_tree_attention_paged(q, c.k[0], c.v[0], c.table, kp, vp, cu, c.len, P,
+                                                parent=np.concatenate(parents))
+    assert _lib.device_error() == 0
+    _check_tree(got, c, q, kp, vp, [_seen(p) for p in parents], cu, S, dt, 0.0 if dtype == "fp32" else _half(dt))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_tree_strides_of_four_elements(cuda, dtype):
+    # head strides that are multiples of 4 but not of 8: the CUDA-core form, products in 32 bits throughout
+    S, P = [200, 13], [20, 65]
+    dt = TYPES[dtype]
+    c, q, kp, vp, parents, cu = _tree_inputs(cuda, 29, S, P, 8, 2, 128, 24, dt)
+    wide = torch.zeros(q.shape[0], 8, 132, dtype=dt, device=cuda)
+    wide[..., :128] = q
+    got = cast_b200.varlen_tree_attention_paged(wide[..., :128], c.k[0], c.v[0], c.table, kp, vp, cu, c.len, P,
+                                                parent=np.concatenate(parents))
+    assert _lib.device_error() == 0
+    _check_tree(got, c, q, kp, vp, [_seen(p) for p in parents], cu, S, dt, 0.0)
 
 
 @pytest.mark.parametrize("dtype,Hq", [("bf16", 32), ("fp32", 8)])
