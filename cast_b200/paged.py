@@ -79,8 +79,9 @@ def _pages(k_pages, v_pages, name):
 
 
 def _aligned(stride, ptr):
-    """What the attention kernels take: dim stride 1, row / head strides multiples of 4, a 16-byte aligned base."""
-    return stride[2] == 1 and stride[0] % 4 == 0 and stride[1] % 4 == 0 and ptr % 16 == 0
+    """What the attention kernels take: dim stride 1, row / head strides multiples of 4 (not 0), a 16-byte aligned base."""
+    s0, s1, s2 = stride
+    return s2 == 1 and s0 % 4 == 0 and s1 % 4 == 0 and ptr % 16 == 0 and s0 > 0 and s1 > 0
 
 
 def _input(t):
