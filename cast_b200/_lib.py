@@ -1,12 +1,16 @@
 """Loader and build recipe of the in-tree C-ABI library ``libcast_b200.so``.
 
 The library is built by nvcc straight from ``cast_b200/csrc`` for sm_100a
-(``build()``) and loaded with ctypes. There is no CPU fallback: every entry
+(``build()``) and loaded with ctypes. ``_paged_binding.so`` beside it (g++,
+``build_binding()``) calls the paged entry points without ctypes. There is no CPU fallback: every entry
 point in this package raises if the library or a CUDA device is missing.
 """
 import ctypes
+import importlib.util
 import os
+import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -14,6 +18,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB_PATH = Path(os.environ["CAST_B200_LIB"]) if os.environ.get("CAST_B200_LIB") else PKG / "libcast_b200.so"
 HEADER = ROOT / "include" / "cast_b200.h"
+BINDING_SOURCE = CSRC / "paged_binding.cpp"
+BINDING_PATH = PKG / "_paged_binding.so"
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared"]
@@ -66,6 +72,47 @@ def build(force=False, verbose=False):
     if verbose:
         print(res.stderr)
     return LIB_PATH
+
+
+def build_binding(force=False):
+    """Compile csrc/paged_binding.cpp against Python and the installed torch."""
+    if not force and BINDING_PATH.exists() and all(BINDING_PATH.stat().st_mtime >= s.stat().st_mtime
+                                                   for s in (BINDING_SOURCE, HEADER)):
+        return BINDING_PATH
+    import torch
+    t = Path(torch.__file__).resolve().parent
+    cuda = Path(shutil.which(os.environ.get("NVCC", "nvcc")) or "/usr/local/cuda/bin/nvcc").resolve().parents[1]
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{d}" for d in (t / "include", t / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
+                                cuda / "include")],
+           str(BINDING_SOURCE), "-o", str(tmp), f"-L{t / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+           "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed ({res.returncode}):\n{res.stderr}")
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
+
+
+_BINDING = None
+
+
+def binding():
+    """The loaded binding of the paged entry points (builds it if stale)."""
+    global _BINDING
+    if _BINDING is None:
+        import torch  # noqa: F401  (its libraries are the binding's)
+        L = lib()
+        spec = importlib.util.spec_from_file_location("_paged_binding", build_binding())
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind(*[ctypes.cast(f, ctypes.c_void_p).value for f in (
+            L.cast_paged_append, L.cast_paged_decode_attn, L.cast_paged_decode_workspace_size,
+            L.cast_tree_attn_paged_fwd, L.cast_tree_attn_paged_workspace_size)])
+        _BINDING = mod
+    return _BINDING
 
 
 _LIB = None

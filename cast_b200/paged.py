@@ -19,6 +19,9 @@ and a verify round of draft trees, whose accepted rows are appended for every la
                  accepted=walk.accepted)
 
 A length or page id out of range is skipped on the device and reported by ``_lib.device_error()``.
+
+Each call first goes to the binding (``csrc/paged_binding.cpp``), which takes arguments that are already as the C ABI
+wants them; everything else (conversions, copies, refusals) is done here.
 """
 import struct
 from functools import lru_cache
@@ -148,6 +151,10 @@ def append_paged(k_pages, v_pages, page_table, seq_len, k, v, cu_q=None, *, keep
     position is the slot, or ``positions`` [total]. q: [total, H_q, D], turned likewise into ``q_out`` (a new
     tensor unless given; may be q itself), which is returned. Rows that are not appended are not written.
     """
+    done = (_lib._BINDING or _lib.binding()).append(k_pages, v_pages, page_table, seq_len, k, v, cu_q, keep, accepted,
+                                                    inv_freq, positions, interleaved, rope_scale, q, q_out)
+    if done is not NotImplemented:
+        return done
     many = isinstance(k_pages, (list, tuple))
     kps, vps, ks, vs = (k_pages, v_pages, k, v) if many else ((k_pages,), (v_pages,), (k,), (v,))
     n = len(kps)
@@ -238,6 +245,10 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     float32, bfloat16 or float16, D 64 or 128, any H_q / H_kv. The key ranges of all sequences are split evenly
     over the GPU, whatever their lengths; results do not depend on timing.
     """
+    done = (_lib._BINDING or _lib.binding()).decode(q, k_pages, v_pages, page_table, seq_len, sm_scale, softcap, window,
+                                                    alibi_slopes, out, lse, workspace)
+    if done is not NotImplemented:
+        return done
     (num_pages, H_kv, ps, D), sp, dtype, index = _pages(k_pages, v_pages, "decode_attention_paged")
     shape = q.shape
     if len(shape) != 3 or shape[2] != D or q.dtype is not dtype or q.get_device() != index:
@@ -286,6 +297,11 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
     pages, whatever their size; float32 on the exact CUDA-core kernel. D 64 or 128.
     max_pack / max_prefix bound pack_len and prefix_len; given, the call reads nothing back to the host.
     """
+    done = (_lib._BINDING or _lib.binding()).tree(q, k_pages, v_pages, page_table, k_pack, v_pack, cu_q, prefix_len,
+                                                  pack_len, ancestor_mask, sm_scale, parent, max_pack, max_prefix, out,
+                                                  workspace)
+    if done is not NotImplemented:
+        return done
     (num_pages, H_kv, ps, D), sp, dtype, index = _pages(k_pages, v_pages, "varlen_tree_attention_paged")
     shape = q.shape
     total_q, H_q, _ = shape

@@ -111,3 +111,18 @@ def test_python_refusals():
     with pytest.raises(ValueError, match="per layer"):
         cast_b200.append_paged([pages], [pages], table, length, [row, row], [row])
     assert cast_b200.append_paged([], [], table, length, [], []) is None
+
+
+def test_binding_leaves_what_it_does_not_take():
+    # no CUDA tensor, too few arguments, no tensor at all: paged.py goes on (and refuses above)
+    b = _lib.binding()
+    pages, row, ints = torch.zeros(4, 2, 16, 64), torch.zeros(1, 2, 64), torch.zeros(1, 2, dtype=torch.int32)
+    args = (pages, pages, ints, ints[0], row, row, None, None, None, None, None, False, 1.0, None, None)
+    assert b.append(*args) is NotImplemented
+    assert b.append(*args[:5]) is NotImplemented and b.decode() is NotImplemented and b.tree(None) is NotImplemented
+    assert b.append([], [], ints, ints, [], [], *args[6:]) is NotImplemented
+    assert b.decode(*[3] * 12) is NotImplemented and b.tree(*[None] * 16) is NotImplemented
+    with pytest.raises(TypeError):
+        b.bind(1)
+    with pytest.raises(TypeError):
+        b.bind(*["x"] * 5)

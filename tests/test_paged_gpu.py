@@ -651,3 +651,66 @@ def test_prompt_verify_accept_and_decode_on_one_cache(cuda):
             out, _, e, pv = _attend(qr[b:b + 1], kk, vv, 1 / math.sqrt(D), 0, None, None)
             _check_attention(got[b:b + 1], out, e + 2 * _half(dt) * 4, pv, n + 1, dt, 2.0 ** -15)
     assert _lib.device_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ binding
+def test_binding_and_python_path_agree(cuda):
+    """Arguments that need no conversion go through the binding, others (here 64-bit lengths, lists) through paged.py."""
+    b = _lib.binding()
+    c = Cache(41, [90, 0, 33], 2, 128, 16, torch.bfloat16, cuda, room=8, poison=False, layers=2)
+    g = torch.Generator(device=cuda).manual_seed(42)
+    rnd = lambda *s: torch.empty(s, dtype=torch.bfloat16, device=cuda).normal_(generator=g)
+    q, k, v = rnd(3, 8, 128), rnd(3, 2, 128), rnd(3, 2, 128)
+    freq = _freq(128, cuda)
+    args = (c.k[0], c.v[0], c.table, c.len, k, v, None, None, None, freq, None, False, 1.0)
+    first = b.append(*args, q, None)
+    assert isinstance(first, torch.Tensor) and b.append(*args, None, None) is None
+    kept = c.k[0].clone(), c.v[0].clone()
+    slow = cast_b200.append_paged(c.k[0], c.v[0], c.table.long(), c.len.tolist(), k, v, inv_freq=freq.double(), q=q)
+    assert torch.equal(first, slow) and torch.equal(kept[0], c.k[0]) and torch.equal(kept[1], c.v[0])
+    lens = c.len + 1
+    one = b.decode(q, c.k[0], c.v[0], c.table, lens, None, 0.0, 0, None, None, None, None)
+    assert torch.equal(one, cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, lens.long()))
+    cu, packs, par = torch.tensor([0, 2, 3, 3], dtype=torch.int32, device=cuda), [2, 1, 0], [-1, 0, -1]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    many = b.tree(q, c.k[0], c.v[0], c.table, k, v, cu, c.len, i32(packs), None, None, i32(par), 2, 90, None, None)
+    slow = cast_b200.varlen_tree_attention_paged(q, c.k[0], c.v[0], c.table, k, v, cu, c.len, packs, parent=par)
+    assert torch.equal(many[:3], slow[:3])
+    keep, acc = i32([[0, 1], [0, -1], [-1, -1]]), i32([2, 1, 0])
+    out = b.append(c.k, c.v, c.table, c.len, [k, k], [v, v], cu, keep, acc, None, None, False, 1.0, None, None)
+    assert out is None
+    kept = [t.clone() for t in c.k + c.v]
+    cast_b200.append_paged(tuple(c.k), tuple(c.v), c.table, c.len, [k, k], [v, v], cu.tolist(), keep=keep, accepted=acc)
+    assert all(torch.equal(x, y) for x, y in zip(kept, c.k + c.v)) and _lib.device_error() == 0
+
+
+def test_refusals_on_the_device(cuda):
+    p = torch.zeros(4, 2, 16, 96, dtype=torch.bfloat16, device=cuda)
+    table, n = torch.zeros(1, 2, dtype=torch.int32, device=cuda), torch.ones(1, dtype=torch.int32, device=cuda)
+    q = torch.zeros(1, 4, 96, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(_lib.CastError, match="head dim"):
+        cast_b200.decode_attention_paged(q, p, p, table, n)
+    r = p[..., :64]
+    q64 = q[..., :64].contiguous()
+    for bad in (dict(softcap=-1.0), dict(window=-1), dict(lse=torch.zeros(1, 3, device=cuda)),
+                dict(alibi_slopes=torch.zeros(3, device=cuda)), dict(out=q64.float())):
+        with pytest.raises(ValueError):
+            cast_b200.decode_attention_paged(q64, r, r, table, n, **bad)
+    with pytest.raises(ValueError):
+        cast_b200.decode_attention_paged(q64, r, r.contiguous(), table, n)          # other strides
+    with pytest.raises(ValueError):
+        cast_b200.decode_attention_paged(q64.float(), r, r, table, n)
+    with pytest.raises(AssertionError):
+        cast_b200.decode_attention_paged(q64[:, :3].contiguous(), r, r, table, n)
+    k = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device=cuda)
+    for bad in (dict(q=q64), dict(keep=table), dict(inv_freq=torch.ones(33, device=cuda)), dict(q_out=q64),
+                dict(positions=torch.zeros(2, device=cuda))):
+        with pytest.raises(ValueError):
+            cast_b200.append_paged(r, r, table, n, k, k, **bad)
+    with pytest.raises(ValueError):
+        cast_b200.append_paged(r, r, table, n, k, k[:, :1])
+    with pytest.raises(ValueError):
+        cast_b200.varlen_tree_attention_paged(q64, r, r, table, k, k, [0, 1], n, n)
+    with pytest.raises(_lib.CastError):
+        cast_b200.append_paged(r, r, table[:, :0], n, k, k)
+    assert _lib.device_error() == 0
