@@ -104,7 +104,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ int ranked_sequence(const AttnParams& p, int rank, int* keys) {
   __shared__ int seq_of_rank;
   const int tid = threadIdx.x, nt = blockDim.x;
-  if (p.B <= kMaxRankedSeqs) {
+  if (p.B > 1 && p.B <= kMaxRankedSeqs) {
     for (int i = tid; i < p.B; i += nt) {
       const long long k = (long long)p.prefix_len[i] + p.pack_len[i];
       keys[i] = (int)max(-1LL, min(k, 0x7fffffffLL));
