@@ -1173,7 +1173,8 @@ cudaError_t launch_append(papp::Args& a, const papp::Layers& ly, bool vec, int n
 
 // Query heads of one KV head that a worker takes together. More are read by several workers at about the same
 // time, the second time from L2: 64 sequences of 4000 keys with 32 heads to a KV head take 58 us in tiles of 16
-// against 69 in one of 32 (whose registers spill), 32-bit 64 / 8 heads 581 us in tiles of 4 against 789 in 8.
+// against 69 in one of 32 (whose registers spill), 32-bit 64 / 8 heads 581 us in tiles of 4 against 789 in 8 (four
+// warps to a CTA then; 52 and 493 us since).
 int decode_rows(int dtype, int G) {
   const int most = dtype == CAST_F32 ? 4 : 16, tiles = (G + most - 1) / most;
   return (G + tiles - 1) / tiles;
@@ -1187,7 +1188,7 @@ struct DecodeLayout {
 DecodeLayout decode_layout(int dtype, int G, int D, int sms) {
   DecodeLayout l;
   l.rows = decode_rows(dtype, G);
-  l.workers = sms * pdec::CTAS_PER_SM * pdec::NW;
+  l.workers = sms * pdec::ctas_per_sm(dtype == CAST_F32 ? 4 : 2) * pdec::NW;
   const size_t slots = 2 * (size_t)l.workers * (1 + pdec::NS) * l.rows;
   l.ml = align256(slots * D * sizeof(float));
   l.total = l.ml + align256(slots * 2 * sizeof(float));

@@ -30,17 +30,20 @@
 namespace cast {
 namespace pdec {
 
-constexpr int NW = 4;            // warps (workers) per CTA
+constexpr int NW = 2;            // warps (workers) per CTA
 constexpr int NT = NW * 32;
 constexpr int NS = 2;            // short tails of a long group,
 constexpr int TAIL = 12;         // each 1 / TAIL of it,
 constexpr int MIN_TAIL = 8;      // and of at least this many steps (tails of 4 cost a sequence of 131072 keys a tenth)
 
-// Keys per step, and ring stages per worker: eight workers per SM (two CTAs) hold 192 KB.
+// Keys per step, CTAs per SM, and ring stages per worker: 192 KB an SM. Two warps to a CTA start tails sooner
+// than four (64 ragged sequences 239 against 244 us). 32-bit: the scores' FMAs want more warps than the
+// copies want stages (64 sequences of 3000 keys, 32 / 8 heads: 250 us with 12 warps of two stages, 296 with 8
+// of three; 16-bit 245 against 239 us).
 template <typename T, int D> __host__ __device__ constexpr int step_keys() { return 4096 / (D * (int)sizeof(T)); }
 template <typename T, int D> __host__ __device__ constexpr int stage_bytes() { return 2 * step_keys<T, D>() * D * (int)sizeof(T); }
-template <typename T, int D> __host__ __device__ constexpr int stages() { return 24 * 1024 / stage_bytes<T, D>(); }
-constexpr int CTAS_PER_SM = 2;
+template <typename T, int D> __host__ __device__ constexpr int stages() { return sizeof(T) == 4 ? 2 : 3; }
+__host__ __device__ constexpr int ctas_per_sm(int elem_bytes) { return elem_bytes == 4 ? 6 : 4; }
 constexpr int JOIN_NT = 256;
 
 struct Params {
@@ -272,7 +275,7 @@ __device__ __forceinline__ Work plan_steps(const Params& p) {
   Work wk;
   Cursor& c = wk.c;
   wk.piece = -1;
-  // the heads' CTAs come first; tail CTA x takes tail x % NS of four neighbouring groups
+  // the heads' CTAs come first; tail CTA x takes tail x % NS of NW neighbouring groups
   const int heads = p.W / NW;
   int g = blockIdx.x * NW + (tid >> 5), j = 0;
   if ((int)blockIdx.x >= heads) {
