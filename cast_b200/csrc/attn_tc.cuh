@@ -455,17 +455,19 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
       if (BY_ROWS) fence_proxy_async_smem();   // rows written by asynchronous copies, read by the MMAs
       return done;
     };
-    // Store mode: the last prefix tile also holds store rows past the prefix; their scores
-    // are masked, but 0 x (a non-finite stale value) would still poison P V, so those V rows
-    // are zeroed (whole 128-byte rows: the swizzle only permutes inside a row).
+    // Prefix in stores or pages: the last prefix tile also holds rows past the prefix, a pack's last tile rows
+    // of the next packs or behind the last one. Their scores are masked, but 0 x (a non-finite value of
+    // another request) would still poison P V, so those V rows are zeroed (whole 128-byte rows: the swizzle
+    // only permutes inside a row). The zeroing runs while the softmax is under way:
+    // one pack of 17 on 512 keys takes 11.3 us with it and without, 64 packs of 128 on 4096-8192 keys 793.
     auto zero_tail = [&](int j, int s) {
       if constexpr (STORE) {
         int n0, klim;
         tile_keys(j, n0, klim);
-        if (n0 < m.S && n0 + BN > m.S) {
+        if (n0 + BN > klim) {
           uint8_t* vt = smem + SMEM_V + s * TILE_BYTES;
-          for (int e = lane; e < (n0 + BN - m.S) * (8 * PANELS); e += 32) {
-            const int r = m.S - n0 + e / (8 * PANELS), c = e % (8 * PANELS);
+          for (int e = lane; e < (n0 + BN - klim) * (8 * PANELS); e += 32) {
+            const int r = klim - n0 + e / (8 * PANELS), c = e % (8 * PANELS);
             *reinterpret_cast<uint4*>(vt + (c >> 3) * HALF_BYTES + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();

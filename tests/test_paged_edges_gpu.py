@@ -1,0 +1,87 @@
+"""Paged cache operators where a value that is no part of a result, or a number at the edge of its type, could reach it.
+
+The helpers and their bounds are those of test_paged_gpu.py.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import cast_b200
+from cast_b200 import _lib
+
+from .test_paged_gpu import TYPES, _tree_inputs
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------- rows of other requests
+# one pack tile holds up to 128 rows from the pack's first: rows of the next packs, and rows behind the last one
+SPLIT = ([3000, 2000, 2500], [17, 20, 40])          # few units: the launch cuts the keys into chunks
+WHOLE = ([0, 128, 300, 64], [9, 1, 130, 64])        # one and two query tiles, one and two pack tiles
+MANY = ([40] * 24, [3] * 24)                        # 192 units of one chunk each
+
+
+def _poisoned(x, value, rows):
+    y = x.clone()
+    y[rows] = value
+    return y
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("S,P", [SPLIT, WHOLE, MANY], ids=["split", "whole", "many"])
+@pytest.mark.parametrize("ps,Hq,Hkv,D", [(16, 8, 2, 128), (1, 8, 2, 128), (24, 12, 4, 64), (3, 6, 2, 64)])
+def test_tree_keeps_other_packs_out(cuda, dtype, S, P, ps, Hq, Hkv, D):
+    dt = TYPES[dtype]
+    c, q, kp, vp, parents, cu = _tree_inputs(cuda, 51, S, P, Hq, Hkv, D, ps, dt)
+    pad = torch.zeros(67, Hkv, D, dtype=dt, device=cuda)
+    kp, vp = torch.cat((kp, pad)), torch.cat((vp, pad))            # 67 rows behind the last pack
+    q = torch.cat((q, torch.zeros(67, Hq, D, dtype=dt, device=cuda)))
+    total = int(cu[-1])
+    par = np.concatenate(parents + [[-1] * 67]).astype(np.int32)
+
+    def run(k, v):
+        out = cast_b200.varlen_tree_attention_paged(q, c.k[0], c.v[0], c.table, k, v, cu, c.len, P, parent=par,
+                                                    out=torch.zeros_like(q))
+        assert _lib.device_error() == 0
+        return out
+
+    good = run(kp, vp)
+    assert torch.isfinite(good).all()
+    behind = slice(total, total + 67)
+    one = slice(int(cu[1]), int(cu[2]))                            # request 1's own rows
+    rest = torch.ones(total, dtype=torch.bool, device=cuda)
+    rest[one] = False
+    for kv, vv in ((math.nan, math.inf), (math.inf, math.nan), (1.0, -math.inf)):
+        got = run(_poisoned(kp, kv, behind), _poisoned(vp, vv, behind))
+        assert torch.equal(got[:total], good[:total])
+        got = run(_poisoned(_poisoned(kp, kv, behind), kv, one), _poisoned(_poisoned(vp, vv, behind), vv, one))
+        assert torch.equal(got[:total][rest], good[:total][rest])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("S,P", [SPLIT, WHOLE, MANY], ids=["split", "whole", "many"])
+def test_store_form_keeps_other_packs_out(cuda, dtype, S, P):
+    dt = TYPES[dtype]
+    g = torch.Generator(device=cuda).manual_seed(52)
+    rnd = lambda *s: torch.empty(s, dtype=dt, device=cuda).normal_(generator=g)
+    B, Hq, Hkv, D, total = len(S), 8, 2, 128, sum(P)
+    ks, vs, q = rnd(B, Hkv, max(S) + 5, D), rnd(B, Hkv, max(S) + 5, D), rnd(total + 67, Hq, D)
+    kp, vp = rnd(total + 67, Hkv, D), rnd(total + 67, Hkv, D)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    cu = np.concatenate([[0], np.cumsum(P)]).tolist()
+    par = i32(sum([[-1] + list(range(p - 1)) for p in P], []) + [-1] * 67)
+
+    def run(k, v):
+        out = cast_b200.varlen_tree_attention_store(q, ks, vs, k, v, i32(cu), i32(S), i32(P), parent=par,
+                                                    out=torch.zeros_like(q))
+        assert _lib.device_error() == 0
+        return out
+
+    good = run(kp, vp)
+    behind, one = slice(total, total + 67), slice(cu[1], cu[2])
+    rest = torch.ones(total, dtype=torch.bool, device=cuda)
+    rest[one] = False
+    got = run(_poisoned(_poisoned(kp, math.nan, behind), math.nan, one), _poisoned(_poisoned(vp, math.inf, behind), math.nan, one))
+    assert torch.equal(got[:total][rest], good[:total][rest])
