@@ -88,10 +88,10 @@ bool integer(PyObject* o, int& x) {
   return true;
 }
 
-// The caller's workspace where it is large enough, else a new one (kept in `own`).
+// The caller's workspace where it is large enough and one piece, else a new one (kept in `own`).
 void* workspace(const at::Tensor* given, size_t n, const at::Tensor& on, at::Tensor& own) {
   if (n == 0) return nullptr;
-  if (given && given->device() == on.device() && given->nbytes() >= n &&
+  if (given && given->device() == on.device() && given->nbytes() >= n && given->is_contiguous() &&
       reinterpret_cast<uintptr_t>(given->data_ptr()) % 256 == 0)
     return given->data_ptr();
   own = at::empty({static_cast<int64_t>(n)}, on.options().dtype(at::kByte));

@@ -122,10 +122,12 @@ def _tree_bytes(index, *args):
 
 
 def _workspace(workspace, n, index):
-    """The caller's workspace where it is large enough and on device `index`, else a new one (None: nothing is needed)."""
+    """The caller's workspace where it is large enough, one piece and on device `index`, else a new one (None: nothing is
+    needed). A view with gaps or repeats has other, or fewer, bytes behind its address than it counts."""
     if n == 0:
         return None
-    if workspace is None or workspace.nbytes < n or workspace.data_ptr() % 256 or workspace.get_device() != index:
+    if workspace is None or workspace.nbytes < n or workspace.data_ptr() % 256 or workspace.get_device() != index \
+            or not workspace.is_contiguous():
         return torch.empty(n, dtype=torch.uint8, device=index)
     return workspace
 

@@ -77,6 +77,15 @@ def attention_plan(q, k, v, out, B, max_pack, max_kv, fp32_path="split"):
     return {0: "simt", 1: "tcgen05", 2: "tcgen05_split"}[plan[0]], int(plan[1]), int(plan[2])
 
 
+def _workspace(workspace, n, dev):
+    """The caller's workspace where its n bytes are one piece on `dev`, else a new one. A view with gaps or repeats has
+    other, or fewer, bytes behind its address than it counts."""
+    if n > 0 and (workspace is None or workspace.numel() * workspace.element_size() < n or workspace.data_ptr() % 256 != 0
+                  or workspace.device != dev or not workspace.is_contiguous()):
+        return torch.empty(n, dtype=torch.uint8, device=dev)
+    return workspace
+
+
 def varlen_tree_attention(q, k, v, cu_q, cu_kv, prefix_len, pack_len, ancestor_mask=None, sm_scale=None,
                           *, parent=None, max_pack=None, max_kv=None, out=None, workspace=None, fp32_path="split"):
     """q: [total_q, H_q, D], k/v: [total_kv, H_kv, D] -> [total_q, H_q, D] (q's dtype).
@@ -120,9 +129,7 @@ def varlen_tree_attention(q, k, v, cu_q, cu_kv, prefix_len, pack_len, ancestor_m
     dcode = _code(q.dtype, D, H_q // H_kv, fp32_path)
     ws_bytes = int(_lib.lib().cast_tree_attn_workspace_size_kv(dcode, B, total_q, total_kv, H_q, H_kv, D,
                                                                max_pack, max_kv))
-    if ws_bytes > 0 and (workspace is None or workspace.numel() * workspace.element_size() < ws_bytes
-                         or workspace.data_ptr() % 256 != 0):
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    workspace = _workspace(workspace, ws_bytes, dev)
     strides = (ctypes.c_int64 * 12)(*q.stride(), *k.stride(), *v.stride(), *out.stride())
     stream = torch.cuda.current_stream(dev).cuda_stream
     code = _lib.lib().cast_tree_attn_fwd(
@@ -219,9 +226,7 @@ def varlen_tree_attention_store(q, k_store, v_store, k_pack, v_pack, cu_q, prefi
         par = _i32(parent, dev)
         par_ptr = par.data_ptr()
     ws_bytes = int(L.cast_tree_attn_store_workspace_size(code, B, total_q, H_q, H_kv, D, max_pack, max_prefix))
-    if ws_bytes > 0 and (workspace is None or workspace.numel() * workspace.element_size() < ws_bytes
-                         or workspace.data_ptr() % 256 != 0):
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    workspace = _workspace(workspace, ws_bytes, dev)
     strides = (ctypes.c_int64 * 20)(*q.stride(), *k_store.stride(), *v_store.stride(), *k_pack.stride(),
                                     *v_pack.stride(), *out.stride())
     code = L.cast_tree_attn_store_fwd(

@@ -85,3 +85,32 @@ def test_store_form_keeps_other_packs_out(cuda, dtype, S, P):
     rest[one] = False
     got = run(_poisoned(_poisoned(kp, math.nan, behind), math.nan, one), _poisoned(_poisoned(vp, math.inf, behind), math.nan, one))
     assert torch.equal(got[:total][rest], good[:total][rest])
+
+
+# ------------------------------------------------------------------------------------- workspaces
+def test_workspaces_with_gaps_or_repeats(cuda):
+    """A workspace view that is not one piece is left alone: a new one is taken, the bytes between its own stay."""
+    c, q, kp, vp, parents, cu = _tree_inputs(cuda, 57, [3000, 2000], [17, 20], 8, 2, 128, 16, torch.bfloat16)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    par, P = i32(sum(parents, [])), i32([17, 20])
+    ks, vs = (torch.stack([torch.nn.functional.pad(c.rows(pg, b, 0, n), (0, 0, 0, 0, 0, 3000 - n)).transpose(0, 1).contiguous()
+                           for b, n in enumerate(c.lens)]) for pg in (c.k[0], c.v[0]))
+    k, v = (torch.cat([t for b, n in enumerate(c.lens) for t in (c.rows(pg, b, 0, n), pk[cu[b]:cu[b + 1]])])
+            for pg, pk in ((c.k[0], kp), (c.v[0], vp)))
+    cu = i32(cu.tolist())
+    calls = [
+        lambda w: cast_b200.decode_attention_paged(q[:2], c.k[0], c.v[0], c.table, c.len, workspace=w),
+        lambda w: cast_b200.decode_attention_paged(q[:2], c.k[0], c.v[0], c.table, c.len.long(), workspace=w),
+        lambda w: cast_b200.varlen_tree_attention_paged(q, c.k[0], c.v[0], c.table, kp, vp, cu, c.len, P, parent=par,
+                                                        max_pack=20, max_prefix=3000, workspace=w),
+        lambda w: cast_b200.varlen_tree_attention_store(q, ks, vs, kp, vp, cu, c.len, P, parent=par, workspace=w),
+        lambda w: cast_b200.varlen_tree_attention(q, k, v, cu, i32([0, 3017, 5037]), c.len, P, parent=par, workspace=w),
+    ]
+    big = torch.full((64 << 20,), 7, dtype=torch.uint8, device=cuda)
+    for call in calls:
+        want = call(None)
+        for view in (big[:1].expand(32 << 20), big[::2]):
+            assert torch.equal(call(view), want)
+        assert (big == 7).all() and _lib.device_error() == 0
+        assert torch.equal(call(big), want) and not (big == 7).all()      # one piece: used
+        big.fill_(7)
