@@ -384,12 +384,14 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const AttnParams p) {
   } else {
     m = load_seq(p.cu_q, p.cu_kv, p.prefix_len, p.pack_len, b, p.total_q, p.total_kv, p.max_pack, p.max_kv);
   }
-  if (!m.ok || t < m.q0 || t >= m.q0 + m.P) return;
   const int tiles_per_chunk = p.chunk / 128;
   const int nsplit = p.store_mode ? min(p.n_split, (seq_key_tiles(p, m.S, m.P, 128) + tiles_per_chunk - 1) / tiles_per_chunk)
                                   : min(p.n_split, (m.S + m.P + p.chunk - 1) / p.chunk);
-  // launched beside the kernel that writes the partials (paged layout): wait for it; else no wait
+  // launched beside the kernel that writes the partials (paged layout): wait for it, else no wait. Rows of no
+  // sequence wait as well: a launch whose blocks had all left early would let the next one in the stream start
+  // beside the kernel that still reads the cache.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!m.ok || t < m.q0 || t >= m.q0 + m.P) return;
   // the chunks' maxima a lane each; then the chunks in order, the loads of eight under way at a time
   const int64_t slot0 = (int64_t)t * p.H_q + hq, slots = (int64_t)p.total_q * p.H_q;
   float M = -INFINITY;

@@ -114,3 +114,29 @@ def test_workspaces_with_gaps_or_repeats(cuda):
         assert (big == 7).all() and _lib.device_error() == 0
         assert torch.equal(call(big), want) and not (big == 7).all()      # one piece: used
         big.fill_(7)
+
+
+# ------------------------------------------------------------------------------------- rows of no sequence
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_tree_rows_of_no_sequence_then_another_call(cuda, dtype):
+    """Offsets that give every row to an empty second pack: split launches write nothing, and the calls behind them in the
+    stream (which overwrite the cache and reuse the workspace) are not disturbed."""
+    dt = TYPES[dtype]
+    c, q, kp, vp, parents, cu = _tree_inputs(cuda, 58, [6000, 6000], [17, 20], 8, 2, 128, 16, dt)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    par, cu, P = i32(sum(parents, [])), i32(cu.tolist()), i32([17, 20])
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device=cuda)
+    tree = lambda cu, P, out: cast_b200.varlen_tree_attention_paged(q, c.k[0], c.v[0], c.table, kp, vp, cu, c.len, P, parent=par,
+                                                                    max_pack=20, max_prefix=6000, out=out, workspace=ws)
+    keep_k, keep_v = c.k[0].clone(), c.v[0].clone()
+    good = tree(cu, P, torch.empty_like(q))
+    nowhere, empty = i32([0, 0, 0]), i32([17, 0])
+    for _ in range(20):
+        left = torch.full_like(q, 7.0)
+        tree(nowhere, empty, left)
+        c.k[0].fill_(3.0)
+        c.v[0].fill_(3.0)
+        c.k[0].copy_(keep_k)
+        c.v[0].copy_(keep_v)
+        assert torch.equal(tree(cu, P, torch.empty_like(q)), good) and (left == 7.0).all()
+    assert _lib.device_error() == 0
