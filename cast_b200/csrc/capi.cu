@@ -1137,6 +1137,10 @@ int cast_gather_cache(int n_layers, const void* const* src_kv, void* const* dst_
 namespace cast {
 namespace {
 
+// Most keys of a sequence (and rows of a page) that the attention kernels take: key and table indexes are 32-bit, and
+// the copies look up to 4224 keys ahead.
+constexpr int kMaxPagedKeys = 0x7fffffff - 8192;
+
 // Pages [num_pages, H_kv, page_size, D]: strides (page, head, row) that keep every row 16-byte aligned.
 bool page_strides_ok(const int64_t* st, int elem_bytes) {
   for (int i = 0; i < 3; ++i)
@@ -1317,7 +1321,8 @@ int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pag
                            size_t workspace_bytes, cast_stream_t stream) {
   if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return CAST_ERR_DTYPE;
   if (B < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || num_pages < 1 || page_size < 1 || max_pages < 0 ||
-      table_stride < 0 || window < 0 || !(softcap == 0.f || (softcap >= 1e-6f && softcap <= 1e30f)))
+      page_size > kMaxPagedKeys || table_stride < 0 || window < 0 ||
+      !(softcap == 0.f || (softcap >= 1e-6f && softcap <= 1e30f)))
     return CAST_ERR_SHAPE;
   if (D != 64 && D != 128) return CAST_ERR_HEAD_DIM;
   if (B == 0) return CAST_OK;
@@ -1375,6 +1380,7 @@ size_t cast_tree_attn_paged_workspace_size(int dtype, int B, int total_q, int H_
                                            int max_prefix) {
   if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return 0;
   if (B <= 0 || total_q <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || (D != 64 && D != 128)) return 0;
+  if (max_pack < 0 || max_pack > CAST_MAX_PACK || max_prefix < 0 || (int64_t)max_prefix + max_pack > kMaxPagedKeys) return 0;
   const int sms = sm_count();
   const size_t ws = plan_simt(B, total_q, H_q, H_kv, D, max_pack, max_prefix + max_pack, sms, true).ws_bytes;
   if (dtype == CAST_F32 || H_q / H_kv > tca::BM) return ws;
@@ -1390,8 +1396,8 @@ int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_p
                              void* workspace, size_t workspace_bytes, cast_stream_t stream) {
   if (dtype != CAST_F32 && dtype != CAST_BF16 && dtype != CAST_F16) return CAST_ERR_DTYPE;
   if (B < 0 || total_q < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || max_pack < 0 || max_prefix < 0 ||
-      num_pages < 1 || page_size < 1 || max_pages < 0 || table_stride < 0 ||
-      (int64_t)max_prefix + max_pack > 0x7fffffffLL - 256)
+      num_pages < 1 || page_size < 1 || page_size > kMaxPagedKeys || max_pages < 0 || table_stride < 0 ||
+      (int64_t)max_prefix + max_pack > kMaxPagedKeys)
     return CAST_ERR_SHAPE;
   if (D != 64 && D != 128) return CAST_ERR_HEAD_DIM;
   if (max_pack > CAST_MAX_PACK) return CAST_ERR_PACK;

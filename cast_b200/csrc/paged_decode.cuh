@@ -72,8 +72,8 @@ struct Span {
 };
 template <int KS> __device__ __forceinline__ Span span_of(const Params& p, int len) {
   Span z;
-  // out of range (reported by plan_steps): nothing is visible
-  if (len < 0 || len > 0x7fffffff - KS || (int64_t)len > (int64_t)p.max_pages * p.page_size) len = 0;
+  // out of range (reported by plan_steps): nothing is visible. The copies look at table entries up to 63 ahead.
+  if (len < 0 || len > 0x7fffffff - 8192 || (int64_t)len > (int64_t)p.max_pages * p.page_size) len = 0;
   z.len = len;
   z.lo = (p.window > 0 && len > p.window) ? len - p.window : 0;
   z.s0 = z.lo / KS;

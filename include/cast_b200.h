@@ -405,7 +405,8 @@ int cast_gather_cache(int n_layers, const void* const* src_kv, void* const* dst_
  * rows hold max_pages int32 entries; only entries that cover a sequence's keys are
  * read. Two sequences may share pages. A length outside [0, max_pages * page_size]
  * or a page id outside [0, num_pages) is reported as CAST_DEV_BAD_LAYOUT and never
- * read or written through; that sequence's results are then undefined.
+ * read or written through; that sequence's results are then undefined. The attention
+ * calls take sequences and pages of up to 2^31 - 8193 keys.
  */
 
 /*
