@@ -713,8 +713,11 @@ __global__ void __launch_bounds__(NT) decode_f32_kernel(const Params p) {
 #pragma unroll
       for (int i = 1; i < KS; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
       const float mn = fmaxf(m[a], mx);
-      const float al = mn == -INFINITY ? 1.f : exp2f(m[a] - mn);
-      const float pv = mn == -INFINITY ? 0.f : exp2f(s[a] - mn);
+      // the maximum ignores NaN, the probabilities must not: with nothing but hidden and NaN scores so far, 0 is
+      // subtracted, and a NaN reaches the sum and the output
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float al = exp2f(m[a] - mu);
+      const float pv = exp2f(s[a] - mu);
       m[a] = mn;
       l[a] = l[a] * al + pv;            // this lane's key; joined at the end of the unit
 #pragma unroll

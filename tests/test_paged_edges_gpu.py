@@ -11,7 +11,7 @@ import torch
 import cast_b200
 from cast_b200 import _lib
 
-from .test_paged_gpu import TYPES, _tree_inputs
+from .test_paged_gpu import TYPES, Cache, _tree_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +140,45 @@ def test_tree_rows_of_no_sequence_then_another_call(cuda, dtype):
         c.v[0].copy_(keep_v)
         assert torch.equal(tree(cu, P, torch.empty_like(q)), good) and (left == 7.0).all()
     assert _lib.device_error() == 0
+
+
+# ------------------------------------------------------------------------------------- visible NaN
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 2), (64, 12, 4), (128, 5, 1)])
+def test_decode_shows_every_visible_nan(cuda, dtype, D, Hq, Hkv):
+    """NaN in a query head, in the only key, in a whole first step, in every key, in the last key, in a value: rows of that
+    head group (that dim) are NaN and their log-sum-exp too (not for a value), all others keep their bits."""
+    G = Hq // Hkv
+    lens = [700, 1, 700, 40, 5000, 300]
+    c = Cache(53, lens, Hkv, D, 16, TYPES[dtype], cuda)
+    g = torch.Generator(device=cuda).manual_seed(54)
+    q = torch.empty((len(lens), Hq, D), device=cuda).normal_(generator=g).to(TYPES[dtype])
+
+    def run(q):
+        lse = torch.zeros(len(lens), Hq, device=cuda)
+        out = cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, c.len, lse=lse)
+        assert _lib.device_error() == 0
+        return out, lse
+
+    good, good_lse = run(q)
+    assert torch.isfinite(good).all() and torch.isfinite(good_lse).all()
+    bad = torch.zeros(len(lens), Hq, dtype=torch.bool, device=cuda)
+    q2 = q.clone()
+    q2[0, Hq - 1, 3] = math.nan
+    bad[0, Hq - 1] = True
+
+    def spoil(pages, b, h, n, d):
+        pages[int(c.table[b, n // 16]), h, n % 16, d] = math.nan
+
+    last = Hkv - 1
+    for b, keys in ((1, [0]), (2, range(32)), (3, range(40)), (4, [4999])):
+        for n in keys:
+            spoil(c.k[0], b, last, n, 7)
+        bad[b, last * G:] = True
+    spoil(c.v[0], 5, 0, 17, 11)
+    out, lse = run(q2)
+    assert out[bad].isnan().all() and lse[bad].isnan().all()
+    assert out[5, :G, 11].isnan().all()
+    keep = ~bad[..., None].expand_as(out).clone()
+    keep[5, :G, 11] = False
+    assert torch.equal(out[keep], good[keep]) and torch.equal(lse[~bad], good_lse[~bad])
