@@ -1355,6 +1355,7 @@ int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pag
   p.modified = softcap > 0.f || alibi_slopes != nullptr;
   p.v_minus_k = static_cast<const char*>(v_pages) - static_cast<const char*>(k_pages);
   p.cap_exp = softcap > 0.f ? 2.f * kLog2e / softcap : 0.f;
+  p.cap_inv = softcap > 0.f ? 1.f / softcap : 0.f;
   p.W = lay.workers;
   // tails only where the table has room for groups long enough to be cut: their CTAs take 2 us to find
   // that there is nothing for them

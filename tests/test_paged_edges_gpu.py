@@ -11,7 +11,7 @@ import torch
 import cast_b200
 from cast_b200 import _lib
 
-from .test_paged_gpu import TYPES, Cache, _tree_inputs
+from .test_paged_gpu import TYPES, U32, Cache, _attend, _check_attention, _tree_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -182,3 +182,33 @@ def test_decode_shows_every_visible_nan(cuda, dtype, D, Hq, Hkv):
     keep = ~bad[..., None].expand_as(out).clone()
     keep[5, :G, 11] = False
     assert torch.equal(out[keep], good[keep]) and torch.equal(lse[~bad], good_lse[~bad])
+
+
+# ------------------------------------------------------------------------------------- caps
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("cap", [1e-3, 1.0, 50.0, 1e3, 1e4, 1e6, 1e8, 1e30])
+def test_decode_cap_of_any_size(cuda, dtype, cap):
+    """cap tanh(s / cap) is s itself where the cap is large. Its error goes by the score, not by the cap: 2^-19 of the capped
+    score (below a quarter of the cap a polynomial off by some 2^-22; above it an exponential and a reciprocal of 2^-22 and
+    2^-23, together under 2.5 x 2^-23 of the cap, of which the score has tanh(1/4) or more)."""
+    lens, Hq, Hkv, D = [1, 40, 700, 3000], 8, 2, 128
+    dt = TYPES[dtype]
+    c = Cache(55, lens, Hkv, D, 16, dt, cuda)
+    g = torch.Generator(device=cuda).manual_seed(56)
+    q = (torch.empty((len(lens), Hq, D), device=cuda).normal_(generator=g) * 3).to(dt)
+    lse = torch.zeros(len(lens), Hq, device=cuda)
+    got = cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, c.len, softcap=cap, lse=lse)
+    assert _lib.device_error() == 0
+    for b, n in enumerate(lens):
+        k, v = c.rows(c.k[0], b, 0, n), c.rows(c.v[0], b, 0, n)
+        _, _, e, _ = _attend(q[b:b + 1], k, v, 1 / math.sqrt(D), 0, None, None)      # the dot products' error
+        kk = k.double().repeat_interleave(Hq // Hkv, 1)
+        s = torch.einsum("hd,nhd->hn", q[b].double(), kk) / math.sqrt(D)
+        s = cap * torch.tanh(s / cap)
+        e = e + 2.0 ** -19 * s.abs().amax(-1)
+        p = torch.softmax(s, -1)
+        vv = v.double().repeat_interleave(Hq // Hkv, 1)
+        want, pv = torch.einsum("hn,nhd->hd", p, vv)[None], torch.einsum("hn,nhd->hd", p, vv.abs())[None]
+        _check_attention(got[b:b + 1], want, e, pv, n, dt, 0.0 if dtype == "fp32" else 2.0 ** -15)
+        want_l = torch.logsumexp(s, -1)
+        assert ((lse[b].double() - want_l).abs() <= 2 * e[0] + 2.0 ** -20 + n * U32 + 4 * U32 * want_l.abs()).all()
