@@ -20,7 +20,8 @@
 // 16-bit types: S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16, so that keys and head dims fill the 16
 // rows and the KV head's query heads are the 8 columns (NH tiles of them; with heads as rows a group of 4
 // left 12 of 16 rows idle and held twice the registers). The probabilities are carried as two 16-bit
-// terms (p = hi + lo): the loop is bound by memory, and the only rounding of consequence is the output's.
+// terms (p = hi + lo, in half precision of 2^14 p): the loop is bound by memory, and the only rounding of
+// consequence is the output's.
 // 32-bit: FMAs on the CUDA cores.
 #pragma once
 
@@ -151,7 +152,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// Two probabilities as hi + lo pairs of 16-bit terms.
+// The power of two that probabilities (1 at most) are multiplied by before they are split, and what takes it out
+// of the sums of values again. Half precision ends at 2^-24: one split of p itself lost a sixth of p = 1.4e-7 and
+// everything under 2^-25. Of 2^14 p the two terms are off by 2^-22 p or 2^-39, whichever is more, so 2^17 keys
+// together by 2^-22 of the largest.
+template <typename T> __host__ __device__ constexpr float p_scale() { return std::is_same<T, __half>::value ? 16384.f : 1.f; }
+
+// Two probabilities, scaled, as hi + lo pairs of 16-bit terms.
 template <typename T> __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
@@ -160,6 +167,8 @@ template <typename T> __device__ __forceinline__ void split2(float p0, float p1,
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&r);
   } else {
+    p0 *= p_scale<T>();
+    p1 *= p_scale<T>();
     const __half2 h = __floats2half2_rn(p0, p1);
     const float2 f = __half22float2(h);
     const __half2 r = __floats2half2_rn(p0 - f.x, p1 - f.y);
@@ -602,7 +611,7 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
           const int r = a * 8 + t * 2 + i;
           if (r >= nrow) continue;
           if (direct) {
-            const float inv = lt == 0.f ? 0.f : 1.f / lt;
+            const float inv = lt == 0.f ? 0.f : (1.f / p_scale<T>()) / lt;
             T* out = static_cast<T*>(p.out) + (int64_t)cc.b * p.so_b + (int64_t)(h0 + r) * p.so_h + g;
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
@@ -614,8 +623,8 @@ __global__ void __launch_bounds__(NT) decode_mma_kernel(const Params p) {
             float* wo = p.ws_o + ((int64_t)slot * p.rows + r) * D + g;
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
-              wo[j * 16] = o[a][j][i];
-              wo[j * 16 + 8] = o[a][j][2 + i];
+              wo[j * 16] = o[a][j][i] * (1.f / p_scale<T>());
+              wo[j * 16 + 8] = o[a][j][2 + i] * (1.f / p_scale<T>());
             }
             if (g == 0) *reinterpret_cast<float2*>(p.ws_ml + ((int64_t)slot * p.rows + r) * 2) = make_float2(m[a][i], lt);
           }

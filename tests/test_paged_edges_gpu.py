@@ -212,3 +212,30 @@ def test_decode_cap_of_any_size(cuda, dtype, cap):
         _check_attention(got[b:b + 1], want, e, pv, n, dt, 0.0 if dtype == "fp32" else 2.0 ** -15)
         want_l = torch.logsumexp(s, -1)
         assert ((lse[b].double() - want_l).abs() <= 2 * e[0] + 2.0 ** -20 + n * U32 + 4 * U32 * want_l.abs()).all()
+
+
+# ------------------------------------------------------------------------------------- small probabilities
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,Hq,Hkv,n", [(64, 16, 8, 16000), (128, 8, 4, 16000), (64, 32, 2, 40000)])
+def test_decode_long_tail_of_small_probabilities(cuda, dtype, D, Hq, Hkv, n):
+    """Every 500th key has the score 0 and a value of 0, the others one score near -15.76 (p = 2.4 x 2^-24 of the largest)
+    and a value of 1000: the output is all tail. The two 16-bit terms of 2^14 p are off by half a step of the smaller one,
+    2^-25 at least in half precision, which is 2^-25 / (2.4 x 2^-10) < 2^-16 of p; by 2^-17 of p in bfloat16."""
+    dt = TYPES[dtype]
+    B, ps = 16, 64
+    pages = -(-n // ps)
+    at = torch.arange(pages * ps, device=cuda).view(pages, 1, ps, 1)
+    top = (at % 500 == 7).expand(pages, Hkv, ps, D)
+    level = torch.tensor(-15.76 / math.sqrt(D), dtype=dt, device=cuda)
+    k = torch.where(top, torch.zeros_like(level), level).contiguous()
+    v = torch.where(top, torch.zeros_like(level), torch.full_like(level, 1000.0)).contiguous()
+    q = torch.ones(B, Hq, D, dtype=dt, device=cuda)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda).repeat(B, 1)      # all sequences share the pages
+    got = cast_b200.decode_attention_paged(q, k, v, table, torch.full((B,), n, dtype=torch.int32, device=cuda))
+    assert _lib.device_error() == 0
+    s = level.double() * math.sqrt(D)
+    tops = len(range(7, n, 500))
+    tail = (n - tops) * torch.exp(s)
+    want = (1000.0 * tail / (tops + tail)).expand(B, Hq, D)
+    e = (D + 2) * 2 * U32 * s.abs().expand(B, Hq)
+    _check_attention(got, want, e, want, n, dt, 2.0 ** -16)
