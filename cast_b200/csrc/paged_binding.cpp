@@ -39,9 +39,10 @@ int dtype_code(const at::Tensor& t) {
   }
 }
 
-// Pages [num_pages, H_kv, page_size, D] on a CUDA device, dim stride 1.
+// Pages [num_pages, H_kv, page_size, D] on a CUDA device, dim stride 1. Sizes above the C ABI's int go to paged.py.
 bool pages_ok(const at::Tensor* t) {
-  return t && t->is_cuda() && t->dim() == 4 && t->stride(3) == 1 && dtype_code(*t) >= 0;
+  return t && t->is_cuda() && t->dim() == 4 && t->stride(3) == 1 && dtype_code(*t) >= 0 && t->size(0) <= INT_MAX &&
+         t->size(1) <= INT_MAX && t->size(2) <= INT_MAX;
 }
 bool alike(const at::Tensor* t, const at::Tensor& o) {
   return t && t->sizes() == o.sizes() && t->strides() == o.strides() && t->scalar_type() == o.scalar_type() &&
@@ -61,7 +62,8 @@ bool ints_ok(const at::Tensor* t, const at::Tensor& on, int64_t n, at::ScalarTyp
   return t && t->scalar_type() == type && t->device() == on.device() && t->is_contiguous() && (n < 0 || t->numel() == n);
 }
 bool table_ok(const at::Tensor* t, const at::Tensor& on) {
-  return t && t->dim() == 2 && t->scalar_type() == at::kInt && t->device() == on.device() && t->stride(1) == 1;
+  return t && t->dim() == 2 && t->scalar_type() == at::kInt && t->device() == on.device() && t->stride(1) == 1 &&
+         t->size(0) <= INT_MAX && t->size(1) <= INT_MAX;
 }
 bool device_current(const at::Tensor& t) { return c10::cuda::current_device() == t.get_device(); }
 const int32_t* ints(const at::Tensor* t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; }

@@ -32,6 +32,8 @@ from . import _lib
 from .tree_attn import _DTYPES
 
 
+_INT_MAX = 0x7fffffff       # the C ABI's int; ctypes would pass the low 32 bits of more
+
 # The device and the stream of a call as plain integers: the objects of torch.cuda.current_stream() take 2 us a call,
 # a tenth of what a one-token step has.
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -78,7 +80,10 @@ def _pages(k_pages, v_pages, name):
                          "dim stride 1")
     if v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype is not dtype or v_pages.get_device() != index:
         raise ValueError(f"{name}: K and V pages need one shape, one dtype, one device and the same strides")
-    return shape, stride, dtype, index
+    num_pages, H, ps, D = shape
+    if ps > _INT_MAX or H > _INT_MAX:
+        raise ValueError(f"{name}: too many heads, or rows of a page")
+    return (min(num_pages, _INT_MAX), H, ps, D), stride, dtype, index      # ids, and so reachable pages, are int32
 
 
 def _aligned(stride, ptr):
@@ -164,8 +169,8 @@ def append_paged(k_pages, v_pages, page_table, seq_len, k, v, cu_q=None, *, keep
         raise ValueError("append_paged: one K and one V of pages and of new rows per layer")
     if n == 0:
         return None
-    shape, sp, dtype, index = _pages(kps[0], vps[0], "append_paged")
-    num_pages, H, ps, D = shape
+    (num_pages, H, ps, D), sp, dtype, index = _pages(kps[0], vps[0], "append_paged")
+    shape = kps[0].shape
     rows, sk, sv = ks[0].shape, ks[0].stride(), vs[0].stride()
     if len(rows) != 3 or rows[1] != H or rows[2] != D or sk[2] != 1 or sv[2] != 1:
         raise ValueError("append_paged: new rows are [total, H_kv, D] of the pages' dtype and device, dim stride 1")
@@ -184,7 +189,7 @@ def append_paged(k_pages, v_pages, page_table, seq_len, k, v, cu_q=None, *, keep
         new += (a.data_ptr(), b.data_ptr())
     total = rows[0]
     table = _table(page_table, index)
-    B, width = table.shape
+    B, width = table.shape[0], min(table.shape[1], _INT_MAX)
     seq_len = _i32(seq_len, index, "seq_len", B)
     p_cu = p_keep = p_acc = p_pos = p_freq = p_q = p_qo = qs = None
     w = n_freq = Hq = 0
@@ -258,7 +263,7 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     B, H_q, _ = shape
     assert H_q % H_kv == 0
     table = _table(page_table, index)
-    rows, width = table.shape
+    rows, width = table.shape[0], min(table.shape[1], _INT_MAX)
     if rows != B:
         raise ValueError("decode_attention_paged: page_table must have one row per sequence")
     seq_len = _i32(seq_len, index, "seq_len", B)
@@ -283,7 +288,7 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     _launch(index, _lib.lib().cast_paged_decode_attn, "cast_paged_decode_attn", p_q, k_pages.data_ptr(),
             v_pages.data_ptr(), p_out, p_lse, code, _I7(sq[0], sq[1], sp[0], sp[1], sp[2], so[0], so[1]),
             table.data_ptr(), table.stride(0), width, seq_len.data_ptr(), B, H_q, H_kv, D, num_pages, ps,
-            0.0 if sm_scale is None else sm_scale, softcap, window, p_slopes,
+            0.0 if sm_scale is None else sm_scale, softcap, min(window, _INT_MAX), p_slopes,
             None if workspace is None else workspace.data_ptr(), n)
     return out
 
@@ -315,13 +320,15 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
     if (ancestor_mask is None) == (parent is None):
         raise ValueError("pass exactly one of ancestor_mask and parent")
     table = _table(page_table, index)
-    B, width = table.shape
+    B, width = table.shape[0], min(table.shape[1], _INT_MAX)
     cu_q = _i32(cu_q, index, "cu_q", B + 1)
     prefix_len, pack_len = _i32(prefix_len, index, "prefix_len", B), _i32(pack_len, index, "pack_len", B)
     if max_pack is None:
         max_pack = int(pack_len.max().item()) if B > 0 else 0
     if max_prefix is None:
         max_prefix = int(prefix_len.max().item()) if B > 0 else 0
+    if max(total_q, max_pack, max_prefix) > _INT_MAX:
+        raise ValueError("varlen_tree_attention_paged: total_q, max_pack and max_prefix must be below 2^31")
     q, sq, p_q = _input(q)
     k_pack, sk, p_k = _input(k_pack)
     v_pack, sv, p_v = _input(v_pack)

@@ -239,3 +239,29 @@ def test_decode_long_tail_of_small_probabilities(cuda, dtype, D, Hq, Hkv, n):
     want = (1000.0 * tail / (tops + tail)).expand(B, Hq, D)
     e = (D + 2) * 2 * U32 * s.abs().expand(B, Hq)
     _check_attention(got, want, e, want, n, dt, 2.0 ** -16)
+
+
+# ------------------------------------------------------------------------------------- numbers above 32 bits
+@pytest.mark.parametrize("convert", [False, True], ids=["binding", "python"])
+def test_windows_and_page_counts_above_32_bits(cuda, convert):
+    """The C ABI takes ints: a window of 2^32 + 5 is no window of 5, and 2^32 + 1 pages are not one."""
+    c = Cache(59, [90, 700], 2, 64, 16, torch.bfloat16, cuda)
+    lens, table = (c.len.long(), c.table.long()) if convert else (c.len, c.table)
+    q = torch.ones(2, 4, 64, dtype=torch.bfloat16, device=cuda)
+    want = cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, c.len)
+    for window in ((1 << 31) - 1, 1 << 31, (1 << 32) + 5, 1 << 70):
+        assert torch.equal(cast_b200.decode_attention_paged(q, c.k[0], c.v[0], table, lens, window=window), want)
+    base = torch.zeros(2, 1, 1, 4, 8, device=cuda)
+    k, v = (x.expand((1 << 32) + 1, 1, 4, 8) for x in base)          # every page is the one behind the view
+    new = torch.ones(1, 1, 8, device=cuda)
+    five, zero = torch.full((1, 1), 5, dtype=torch.int32, device=cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    cast_b200.append_paged(k, v, five.long() if convert else five, zero, new, new)
+    assert (base[:, :, :, 0] == 1).all() and (base[:, :, :, 1:] == 0).all() and _lib.device_error() == 0
+    with pytest.raises((ValueError, _lib.CastError)):
+        cast_b200.append_paged(base[0, :, :, :1].expand(1, 1, 1 << 32, 8), base[1, :, :, :1].expand(1, 1, 1 << 32, 8), five, zero, new, new)
+    one = torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda)
+    pk = torch.ones(2, 2, 64, dtype=torch.bfloat16, device=cuda)
+    for bad in (dict(max_pack=1 << 32, max_prefix=700), dict(max_pack=1, max_prefix=(1 << 32) + 700)):
+        with pytest.raises((ValueError, _lib.CastError)):
+            cast_b200.varlen_tree_attention_paged(q, c.k[0], c.v[0], table, pk, pk, one, c.len, [1, 1], parent=[-1, -1], **bad)
+    assert _lib.device_error() == 0
