@@ -81,6 +81,11 @@ bool number(PyObject* o, double& x) {
   if (x == -1.0 && PyErr_Occurred()) { PyErr_Clear(); return false; }
   return true;
 }
+// A scale: None (0, the C ABI's default) or a positive number.
+bool scale_ok(PyObject* o, double& x) {
+  x = 0.0;
+  return o == Py_None || (number(o, x) && x >= 1e-30 && x <= 1e30);
+}
 bool integer(PyObject* o, int& x) {
   if (!PyLong_Check(o)) return false;
   int over = 0;
@@ -195,9 +200,9 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return not_here();
   const int64_t B = q->size(0), heads = q->size(1), kv = kp->size(1), D = kp->size(3);
   if (kv < 1 || heads % kv != 0 || table->size(0) != B || !ints_ok(len, *kp, B)) return not_here();
-  double scale = 0.0, cap;
+  double scale, cap;
   int window;
-  if ((a[5] != Py_None && !number(a[5], scale)) || !number(a[6], cap) || !integer(a[7], window)) return not_here();
+  if (!scale_ok(a[5], scale) || !number(a[6], cap) || !integer(a[7], window)) return not_here();
   if (slopes && (!ints_ok(slopes, *kp, heads, at::kFloat) || slopes->dim() != 1)) return not_here();
   if (lse && (!ints_ok(lse, *kp, B * heads, at::kFloat) || lse->dim() != 2 || lse->size(1) != heads)) return not_here();
   if (out && (!rows_ok(out, *kp, B, heads) || !aligned_rows(*out))) return not_here();
@@ -242,9 +247,9 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       (anc && (!ints_ok(anc, *kp, -1, at::kLong) || anc->numel() % total != 0)))
     return not_here();
   if (out && (!rows_ok(out, *kp, total, heads) || !aligned_rows(*out))) return not_here();
-  double scale = 0.0;
+  double scale;
   int max_pack, max_prefix;
-  if ((a[10] != Py_None && !number(a[10], scale)) || !integer(a[12], max_pack) || !integer(a[13], max_prefix) ||
+  if (!scale_ok(a[10], scale) || !integer(a[12], max_pack) || !integer(a[13], max_prefix) ||
       max_pack < 0 || max_prefix < 0 || !device_current(*kp))
     return not_here();
   const int code = dtype_code(*kp);

@@ -86,6 +86,15 @@ def _pages(k_pages, v_pages, name):
     return (min(num_pages, _INT_MAX), H, ps, D), stride, dtype, index      # ids, and so reachable pages, are int32
 
 
+def _scale(sm_scale, name):
+    """The scale for the C ABI, which takes what is not positive as 1/sqrt(D): only None means that here."""
+    if sm_scale is None:
+        return 0.0
+    if not 1e-30 <= sm_scale <= 1e30:
+        raise ValueError(f"{name}: sm_scale must be positive (1e-30 to 1e30)")
+    return sm_scale
+
+
 def _aligned(stride, ptr):
     """What the attention kernels take: dim stride 1, row / head strides multiples of 4 (not 0), a 16-byte aligned base."""
     s0, s1, s2 = stride
@@ -246,7 +255,7 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     """Attention of one new token per sequence over its pages: q [B, H_q, D] -> [B, H_q, D].
 
     seq_len: int32 [B], the keys of each sequence, the new token's own among them (0: the row becomes 0).
-    Scores are q . k * sm_scale (default 1/sqrt(D)); ``softcap`` > 0 caps them (softcap * tanh(s / softcap));
+    Scores are q . k * sm_scale (positive; default 1/sqrt(D)); ``softcap`` > 0 caps them (softcap * tanh(s / softcap));
     ``alibi_slopes`` (float32 [H_q]) then adds slope * (key position - newest position); ``window`` > 0 keeps the
     last ``window`` keys. ``lse`` (float32 [B, H_q], contiguous) receives the natural log-sum-exp of the scores.
     float32, bfloat16 or float16, D 64 or 128, any H_q / H_kv. The key ranges of all sequences are split evenly
@@ -269,6 +278,7 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     seq_len = _i32(seq_len, index, "seq_len", B)
     if window < 0 or not (softcap == 0.0 or 1e-6 <= softcap <= 1e30):
         raise ValueError("decode_attention_paged: window must not be negative, softcap 0 or 1e-6 to 1e30")
+    sm_scale = _scale(sm_scale, "decode_attention_paged")
     q, sq, p_q = _input(q)
     out, so, p_out = _output(out, q, shape, dtype, index)
     p_slopes = p_lse = None
@@ -288,7 +298,7 @@ def decode_attention_paged(q, k_pages, v_pages, page_table, seq_len, sm_scale=No
     _launch(index, _lib.lib().cast_paged_decode_attn, "cast_paged_decode_attn", p_q, k_pages.data_ptr(),
             v_pages.data_ptr(), p_out, p_lse, code, _I7(sq[0], sq[1], sp[0], sp[1], sp[2], so[0], so[1]),
             table.data_ptr(), table.stride(0), width, seq_len.data_ptr(), B, H_q, H_kv, D, num_pages, ps,
-            0.0 if sm_scale is None else sm_scale, softcap, min(window, _INT_MAX), p_slopes,
+            sm_scale, softcap, min(window, _INT_MAX), p_slopes,
             None if workspace is None else workspace.data_ptr(), n)
     return out
 
@@ -329,6 +339,7 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
         max_prefix = int(prefix_len.max().item()) if B > 0 else 0
     if max(total_q, max_pack, max_prefix) > _INT_MAX:
         raise ValueError("varlen_tree_attention_paged: total_q, max_pack and max_prefix must be below 2^31")
+    sm_scale = _scale(sm_scale, "varlen_tree_attention_paged")
     q, sq, p_q = _input(q)
     k_pack, sk, p_k = _input(k_pack)
     v_pack, sv, p_v = _input(v_pack)
@@ -352,6 +363,6 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
             v_pages.data_ptr(), p_k, p_v, p_out, code,
             _I11(sq[0], sq[1], sp[0], sp[1], sp[2], sk[0], sk[1], sv[0], sv[1], so[0], so[1]), table.data_ptr(),
             table.stride(0), width, cu_q.data_ptr(), prefix_len.data_ptr(), pack_len.data_ptr(), anc_ptr, wpr, par_ptr,
-            B, total_q, num_pages, ps, H_q, H_kv, D, 0.0 if sm_scale is None else sm_scale, max_pack, max_prefix,
+            B, total_q, num_pages, ps, H_q, H_kv, D, sm_scale, max_pack, max_prefix,
             None if workspace is None else workspace.data_ptr(), n)
     return out

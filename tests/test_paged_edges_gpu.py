@@ -265,3 +265,20 @@ def test_windows_and_page_counts_above_32_bits(cuda, convert):
         with pytest.raises((ValueError, _lib.CastError)):
             cast_b200.varlen_tree_attention_paged(q, c.k[0], c.v[0], table, pk, pk, one, c.len, [1, 1], parent=[-1, -1], **bad)
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("convert", [False, True], ids=["binding", "python"])
+def test_scales_that_are_not_positive(cuda, convert):
+    # the C ABI's "0 or less: the default" is no answer to a caller who asks for 0, a negative scale or NaN
+    c = Cache(60, [90, 700], 2, 64, 16, torch.bfloat16, cuda)
+    q, pk = (torch.ones(2, h, 64, dtype=torch.bfloat16, device=cuda) for h in (4, 2))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    lens = c.len.long() if convert else c.len
+    for scale in (0.0, 0, -0.125, math.nan, math.inf, 1e-60):
+        with pytest.raises(ValueError):
+            cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, lens, scale)
+        with pytest.raises(ValueError):
+            cast_b200.varlen_tree_attention_paged(q, c.k[0], c.v[0], c.table, pk, pk, i32([0, 1, 2]), lens, i32([1, 1]), None, scale,
+                                                  parent=i32([-1, -1]), max_pack=1, max_prefix=700)
+    a, b = (cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, lens, s) for s in (None, 0.125))
+    assert torch.equal(a, b) and _lib.device_error() == 0
