@@ -165,7 +165,9 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       fresh = at::empty_like(*q);
       out = &fresh;
     }
-    if (!rows_ok(out, p0, total, q->size(1))) return not_here();
+    if (!rows_ok(out, p0, total, q->size(1)) || (out->stride(0) == 0 && total > 1) ||
+        (out->stride(1) == 0 && out->size(1) > 1))      // rows or heads that fall on one another
+      return not_here();
   }
   const int64_t ps[6] = {p0.stride(0), p0.stride(1), p0.stride(2), p0.stride(0), p0.stride(1), p0.stride(2)};
   const int64_t ns[4] = {k0.stride(0), k0.stride(1), v0.stride(0), v0.stride(1)};

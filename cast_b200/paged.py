@@ -232,8 +232,9 @@ def append_paged(k_pages, v_pages, page_table, seq_len, k, v, cu_q=None, *, keep
         if q_out is None:
             q_out = torch.empty_like(q)
         o = q_out.stride()
-        if q_out.shape != shape_q or q_out.dtype is not dtype or q_out.get_device() != index or o[2] != 1:
-            raise ValueError("append_paged: q_out must be like q, dim stride 1")
+        if q_out.shape != shape_q or q_out.dtype is not dtype or q_out.get_device() != index or o[2] != 1 \
+                or (o[0] == 0 and total > 1) or (o[1] == 0 and shape_q[1] > 1):
+            raise ValueError("append_paged: q_out must be like q, dim stride 1, rows and heads apart")
         Hq, p_q, p_qo, qs = shape_q[1], q.data_ptr(), q_out.data_ptr(), _I4(s[0], s[1], o[0], o[1])
     elif q_out is not None:
         raise ValueError("append_paged: q_out without q")

@@ -282,3 +282,21 @@ def test_scales_that_are_not_positive(cuda, convert):
                                                   parent=i32([-1, -1]), max_pack=1, max_prefix=700)
     a, b = (cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, lens, s) for s in (None, 0.125))
     assert torch.equal(a, b) and _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("convert", [False, True], ids=["binding", "python"])
+def test_append_refuses_queries_written_over_one_another(cuda, convert):
+    c = Cache(61, [9, 20, 0], 2, 64, 16, torch.bfloat16, cuda, room=1, poison=False)
+    q, k = torch.ones(3, 4, 64, dtype=torch.bfloat16, device=cuda), torch.ones(3, 2, 64, dtype=torch.bfloat16, device=cuda)
+    lens, freq = c.len.long() if convert else c.len, torch.ones(32, device=cuda)
+    before = c.k[0].clone()
+    for q_out in (q[:1].clone().expand(3, 4, 64), q[:, :1].clone().expand(3, 4, 64)):
+        with pytest.raises(ValueError, match="q_out"):
+            cast_b200.append_paged(c.k[0], c.v[0], c.table, lens, k, k, inv_freq=freq, q=q, q_out=q_out)
+    assert torch.equal(c.k[0], before)
+    # one source row for every query is fine, and so is a single head or row of any stride
+    same = cast_b200.append_paged(c.k[0], c.v[0], c.table, lens, k, k, inv_freq=freq, q=q[:1].expand(3, 4, 64), q_out=torch.empty_like(q))
+    assert torch.equal(same, cast_b200.append_paged(c.k[0], c.v[0], c.table, lens, k, k, inv_freq=freq, q=q, q_out=torch.empty_like(q)))
+    row = torch.empty(3, 64, dtype=q.dtype, device=cuda)[:, None].expand(3, 1, 64)
+    assert cast_b200.append_paged(c.k[0], c.v[0], c.table, lens, k, k, inv_freq=freq, q=q[:, :1], q_out=row) is row
+    assert _lib.device_error() == 0
