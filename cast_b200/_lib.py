@@ -1,8 +1,9 @@
 """Loader and build recipe of the in-tree C-ABI library ``libcast_b200.so``.
 
 The library is built by nvcc straight from ``cast_b200/csrc`` for sm_100a
-(``build()``) and loaded with ctypes. ``_paged_binding.so`` beside it (g++,
-``build_binding()``) calls the paged entry points without ctypes. There is no CPU fallback: every entry
+(``build()``) and loaded with ctypes. ``_paged_binding.*.so`` beside it (g++,
+``build_binding()``) calls the paged entry points without ctypes; where it cannot be built they go through ctypes
+(slower calls, the same kernels). There is no CPU fallback: every entry
 point in this package raises if the library or a CUDA device is missing.
 """
 import ctypes
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sysconfig
+import warnings
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -19,7 +21,6 @@ CSRC = PKG / "csrc"
 LIB_PATH = Path(os.environ["CAST_B200_LIB"]) if os.environ.get("CAST_B200_LIB") else PKG / "libcast_b200.so"
 HEADER = ROOT / "include" / "cast_b200.h"
 BINDING_SOURCE = CSRC / "paged_binding.cpp"
-BINDING_PATH = PKG / "_paged_binding.so"
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared"]
@@ -56,58 +57,86 @@ def needs_build():
     return any(s.stat().st_mtime > t for s in _sources())
 
 
+def _compile(cmd, path):
+    """Runs cmd(temporary file) and moves the result to `path`. The temporary file is this process's own: ranks that
+    build at once each install a whole file. Returns what the compiler printed."""
+    tmp = Path(f"{path}.{os.getpid()}.tmp")
+    args = cmd(str(tmp))
+    try:
+        res = subprocess.run(args, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"{Path(args[0]).name} failed ({res.returncode}):\n{res.stderr}")
+        os.replace(tmp, path)
+    finally:
+        tmp.unlink(missing_ok=True)
+    return res.stderr
+
+
 def build(force=False, verbose=False):
     """Compile csrc/capi.cu (which includes every kernel) into libcast_b200.so."""
     if not force and not needs_build():
         return LIB_PATH
     nvcc = os.environ.get("NVCC", "nvcc")
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [nvcc, *NVCC_FLAGS, "-o", str(tmp), str(CSRC / "capi.cu")]
+    flags = ["-Xptxas=-v", *NVCC_FLAGS] if verbose else NVCC_FLAGS
+    err = _compile(lambda tmp: [nvcc, *flags, "-o", tmp, str(CSRC / "capi.cu")], LIB_PATH)
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stderr}")
-    os.replace(tmp, LIB_PATH)
-    if verbose:
-        print(res.stderr)
+        print(err)
     return LIB_PATH
+
+
+def binding_path():
+    """Where the binding is. It is built against one Python and one torch, so both are in its name."""
+    import torch
+    return PKG / (f"_paged_binding.{sysconfig.get_config_var('SOABI')}-torch{torch.__version__}"
+                  f"-abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}.so")
 
 
 def build_binding(force=False):
     """Compile csrc/paged_binding.cpp against Python and the installed torch."""
-    if not force and BINDING_PATH.exists() and all(BINDING_PATH.stat().st_mtime >= s.stat().st_mtime
-                                                   for s in (BINDING_SOURCE, HEADER)):
-        return BINDING_PATH
+    path = binding_path()
+    if not force and path.exists() and all(path.stat().st_mtime >= s.stat().st_mtime for s in (BINDING_SOURCE, HEADER)):
+        return path
     import torch
     t = Path(torch.__file__).resolve().parent
     cuda = Path(shutil.which(os.environ.get("NVCC", "nvcc")) or "/usr/local/cuda/bin/nvcc").resolve().parents[1]
-    tmp = BINDING_PATH.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{d}" for d in (t / "include", t / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
-                                cuda / "include")],
-           str(BINDING_SOURCE), "-o", str(tmp), f"-L{t / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
-           "-lc10_cuda"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"g++ failed ({res.returncode}):\n{res.stderr}")
-    os.replace(tmp, BINDING_PATH)
-    return BINDING_PATH
+    _compile(lambda tmp: [
+        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *[f"-I{d}" for d in (t / "include", t / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
+                             cuda / "include")],
+        str(BINDING_SOURCE), "-o", tmp, f"-L{t / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+        "-lc10_cuda"], path)
+    return path
+
+
+class _NoBinding:
+    """Takes no call: every one goes on in paged.py, through ctypes."""
+
+    @staticmethod
+    def _leave(*args):
+        return NotImplemented
+
+    append = decode = tree = _leave
 
 
 _BINDING = None
 
 
 def binding():
-    """The loaded binding of the paged entry points (builds it if stale)."""
+    """The loaded binding of the paged entry points (builds it if stale), or one that takes no call where it cannot be
+    built or loaded (no compiler or headers, a directory that cannot be written)."""
     global _BINDING
     if _BINDING is None:
         import torch  # noqa: F401  (its libraries are the binding's)
         L = lib()
-        spec = importlib.util.spec_from_file_location("_paged_binding", build_binding())
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
+        try:
+            spec = importlib.util.spec_from_file_location("_paged_binding", build_binding())
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+        except (OSError, RuntimeError, ImportError) as e:
+            warnings.warn(f"the paged calls go through ctypes, 5 to 20 us a call slower: their binding is missing ({e})")
+            _BINDING = _NoBinding()
+            return _BINDING
         mod.bind(*[ctypes.cast(f, ctypes.c_void_p).value for f in (
             L.cast_paged_append, L.cast_paged_decode_attn, L.cast_paged_decode_workspace_size,
             L.cast_tree_attn_paged_fwd, L.cast_tree_attn_paged_workspace_size)])

@@ -1,8 +1,14 @@
 """Paged cache calls without a GPU: arguments that must not reach a kernel as they are."""
+import os
+import subprocess
+import sysconfig
+from pathlib import Path
+
 import pytest
 import torch
 
-from cast_b200 import paged, tree_attn
+import cast_b200
+from cast_b200 import _lib, paged, tree_attn
 
 from .test_paged_cpu import L, _decode, _tree  # noqa: F401  (L: fixture)
 
@@ -37,3 +43,45 @@ def test_lengths_near_the_end_of_32_bits(L):  # noqa: F811
     assert size(1, 1, 17, 32, 8, 128, 17, most) == 0 and size(1, 1, 17, 32, 8, 128, 17, (1 << 31) - 1) == 0
     assert size(1, 1, 17, 32, 8, 128, -1, 10) == 0 and size(1, 1, 17, 32, 8, 128, 17, -1) == 0
     assert 0 < size(0, 1, 17, 32, 8, 128, 17, 100000) < size(0, 1, 34, 32, 8, 128, 17, 100000)
+
+
+# ------------------------------------------------------------------------------------- building the binding
+def test_binding_is_named_for_its_python_and_torch():
+    name = _lib.build_binding().name
+    assert torch.__version__ in name and sysconfig.get_config_var("SOABI") in name
+
+
+@pytest.mark.parametrize("build", ["build", "build_binding"])
+def test_builds_at_once_do_not_share_a_temporary_file(monkeypatch, tmp_path, build):
+    # whatever a process writes before the last rename is its own; nothing is left when the compiler fails
+    monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "lib.so")
+    monkeypatch.setattr(_lib, "PKG", tmp_path)
+    seen = []
+
+    def run(cmd, **_):
+        out = Path(cmd[cmd.index("-o") + 1])
+        seen.append(out.name)
+        out.write_bytes(b"x")
+        return subprocess.CompletedProcess(cmd, len(seen) - 1, "", "no luck")
+
+    monkeypatch.setattr(subprocess, "run", run)
+    made = getattr(_lib, build)(force=True)
+    assert made.read_bytes() == b"x" and os.listdir(tmp_path) == [made.name]
+    with pytest.raises(RuntimeError, match="no luck"):
+        getattr(_lib, build)(force=True)
+    assert os.listdir(tmp_path) == [made.name] and all(str(os.getpid()) in n for n in seen)
+
+
+def test_calls_go_through_ctypes_where_the_binding_cannot_be_built(monkeypatch, tmp_path):
+    monkeypatch.setattr(_lib, "PKG", tmp_path)
+    monkeypatch.setattr(_lib, "_BINDING", None)
+    monkeypatch.setenv("CXX", str(tmp_path / "no-such-compiler"))
+    pages, row = torch.zeros(4, 2, 16, 64), torch.zeros(1, 2, 64)
+    ints = torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.warns(UserWarning, match="ctypes"):
+        assert cast_b200.append_paged([], [], ints, ints[0, :1], [], []) is None
+    for call in (lambda: cast_b200.append_paged(pages, pages, ints, ints[0, :1], row, row),
+                 lambda: cast_b200.decode_attention_paged(row, pages, pages, ints, ints[0, :1]),
+                 lambda: cast_b200.varlen_tree_attention_paged(row, pages, pages, ints, row, row, [0, 1], [0], [1], parent=[-1])):
+        with pytest.raises(RuntimeError, match="CUDA"):       # paged.py's own check, not the compiler's failure
+            call()

@@ -300,3 +300,30 @@ def test_append_refuses_queries_written_over_one_another(cuda, convert):
     row = torch.empty(3, 64, dtype=q.dtype, device=cuda)[:, None].expand(3, 1, 64)
     assert cast_b200.append_paged(c.k[0], c.v[0], c.table, lens, k, k, inv_freq=freq, q=q[:, :1], q_out=row) is row
     assert _lib.device_error() == 0
+
+
+# ------------------------------------------------------------------------------------- without the binding
+def test_whole_calls_without_the_binding(cuda, monkeypatch):
+    c = Cache(62, [90, 0, 33], 2, 128, 16, torch.bfloat16, cuda, room=8, poison=False, layers=2)
+    g = torch.Generator(device=cuda).manual_seed(63)
+    rnd = lambda *s: torch.empty(s, dtype=torch.bfloat16, device=cuda).normal_(generator=g)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    q, k, v = rnd(3, 8, 128), rnd(3, 2, 128), rnd(3, 2, 128)
+    first = [t.clone() for t in c.k + c.v]
+
+    def everything():
+        for t, f in zip(c.k + c.v, first):
+            t.copy_(f)
+        lse = torch.zeros(3, 8, device=cuda)
+        outs = [cast_b200.append_paged(c.k[0], c.v[0], c.table, c.len, k, v, inv_freq=torch.ones(64, device=cuda), q=q),
+                cast_b200.decode_attention_paged(q, c.k[0], c.v[0], c.table, c.len + 1, 0.2, softcap=30.0, window=50,
+                                                 alibi_slopes=torch.ones(8, device=cuda), lse=lse), lse,
+                cast_b200.varlen_tree_attention_paged(q, c.k[0], c.v[0], c.table, k, v, i32([0, 2, 3, 3]), c.len, i32([2, 1, 0]),
+                                                      parent=i32([-1, 0, -1]), max_pack=2, max_prefix=90)]
+        cast_b200.append_paged(c.k, c.v, c.table, c.len, [k, k], [v, v], i32([0, 2, 3, 3]), keep=i32([[0, 1], [0, -1], [-1, -1]]),
+                               accepted=i32([2, 1, 0]))
+        return outs + [t.clone() for t in c.k + c.v]
+
+    want = everything()
+    monkeypatch.setattr(_lib, "_BINDING", _lib._NoBinding())
+    assert all(torch.equal(a, b) for a, b in zip(everything(), want)) and _lib.device_error() == 0
