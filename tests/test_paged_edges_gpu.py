@@ -327,3 +327,76 @@ def test_whole_calls_without_the_binding(cuda, monkeypatch):
     want = everything()
     monkeypatch.setattr(_lib, "_BINDING", _lib._NoBinding())
     assert all(torch.equal(a, b) for a, b in zip(everything(), want)) and _lib.device_error() == 0
+
+
+# ------------------------------------------------------------------------------------- refusals, both ways
+def _base_calls(dev):
+    """Arguments of one good call of each operator, by name, in the binding's order, and the public function."""
+    c = Cache(64, [9, 40], 2, 64, 16, torch.bfloat16, dev, room=2, poison=False)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    one = lambda *s: torch.ones(s, dtype=torch.bfloat16, device=dev)
+    append = dict(k_pages=c.k[0], v_pages=c.v[0], page_table=c.table, seq_len=c.len, k=one(2, 2, 64), v=one(2, 2, 64), cu_q=None,
+                  keep=None, accepted=None, inv_freq=torch.ones(32, device=dev), positions=None, interleaved=False, rope_scale=1.0,
+                  q=one(2, 4, 64), q_out=None)
+    decode = dict(q=one(2, 4, 64), k_pages=c.k[0], v_pages=c.v[0], page_table=c.table, seq_len=c.len, sm_scale=None, softcap=0.0,
+                  window=0, alibi_slopes=None, out=None, lse=None, workspace=None)
+    tree = dict(q=one(3, 4, 64), k_pages=c.k[0], v_pages=c.v[0], page_table=c.table, k_pack=one(3, 2, 64), v_pack=one(3, 2, 64),
+                cu_q=i32(0, 2, 3), prefix_len=c.len, pack_len=i32(2, 1), ancestor_mask=None, sm_scale=None, parent=i32(-1, 0, -1),
+                max_pack=2, max_prefix=40, out=None, workspace=None)
+    return {"append": (append, cast_b200.append_paged), "decode": (decode, cast_b200.decode_attention_paged),
+            "tree": (tree, cast_b200.varlen_tree_attention_paged)}
+
+
+def _bad(op, dev):
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    z = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device=dev)
+    f = lambda *s: torch.zeros(s, device=dev)
+    pages = [dict(k_pages=z(4, 2, 16, 64)), dict(v_pages=z(1, 2, 16, 64)), dict(k_pages=f(4, 2, 16, 64), v_pages=f(4, 2, 16, 64)),
+             dict(k_pages=z(4, 2, 16), v_pages=z(4, 2, 16)), dict(k_pages=z(4, 2, 16, 128)[..., ::2], v_pages=z(4, 2, 16, 128)[..., ::2]),
+             dict(page_table=i32(1, 2)), dict(page_table=None)]
+    if op == "append":
+        return pages + [
+            dict(seq_len=i32(1, 2, 3)), dict(k=z(2, 3, 64)), dict(v=z(3, 2, 64)), dict(k=z(2, 2, 32)), dict(k=f(2, 2, 64)), dict(k=z(2, 2, 128)[..., ::2]),
+            dict(cu_q=i32(0, 2)), dict(keep=i32(0, 0).view(2, 1)), dict(accepted=i32(1, 1)), dict(keep=i32(0, 0).view(2, 1), accepted=i32(1, 1)),
+            dict(keep=i32(0, 0), accepted=i32(1, 1), cu_q=i32(0, 1, 2), q=None), dict(keep=i32(0, 0).view(2, 1), accepted=i32(1, 1), cu_q=i32(0, 1, 2)),
+            dict(inv_freq=f(33)), dict(inv_freq=None), dict(positions=i32(1)), dict(q=z(3, 4, 64)), dict(q=z(2, 4, 32)), dict(q=f(2, 4, 64)),
+            dict(q_out=z(2, 3, 64)), dict(q=None, q_out=z(2, 4, 64)), dict(q_out=f(2, 4, 64)), dict(q_out=z(2, 4, 128)[..., ::2]),
+            dict(q_out=z(1, 4, 64).expand(2, 4, 64)), dict(q_out=z(2, 1, 64).expand(2, 4, 64)), dict(page_table=i32(0, 1).view(2, 1)[:, :0])]
+    scale = [dict(sm_scale=0.0), dict(sm_scale=-1.0), dict(sm_scale=math.nan)]
+    if op == "decode":
+        return pages + scale + [
+            dict(q=z(3, 4, 64)), dict(q=z(2, 3, 64)), dict(q=f(2, 4, 64)), dict(q=z(2, 4, 32)), dict(q=z(2, 256)), dict(seq_len=i32(1)),
+            dict(softcap=-1.0), dict(softcap=1e31), dict(softcap=math.nan), dict(window=-1), dict(alibi_slopes=f(3)), dict(alibi_slopes=f(2, 2)),
+            dict(out=z(2, 3, 64)), dict(out=f(2, 4, 64)), dict(out=z(2, 4, 66)[..., 1:65]), dict(out=z(1, 4, 64).expand(2, 4, 64)),
+            dict(lse=f(8)), dict(lse=f(4, 2)), dict(lse=z(2, 4)), dict(lse=f(2, 8)[:, ::2]),
+            dict(k_pages=z(4, 2, 16, 96), v_pages=z(4, 2, 16, 96), q=z(2, 4, 96)),
+            dict(k_pages=z(4, 2, 16, 68)[..., :64], v_pages=z(4, 2, 16, 68)[..., :64])]
+    return pages + scale + [
+        dict(q=z(3, 3, 64)), dict(q=f(3, 4, 64)), dict(q=z(4, 4, 64)), dict(k_pack=z(2, 2, 64)), dict(v_pack=z(3, 1, 64)), dict(k_pack=f(3, 2, 64)),
+        dict(cu_q=i32(0, 3)), dict(prefix_len=i32(1)), dict(pack_len=i32(1, 1, 1)), dict(parent=None), dict(parent=i32(-1, 0)),
+        dict(ancestor_mask=torch.ones(3, dtype=torch.int64, device=dev)), dict(parent=None, ancestor_mask=torch.ones(4, dtype=torch.int64, device=dev)),
+        dict(max_pack=-1), dict(max_prefix=-1), dict(max_pack=2000), dict(max_pack=1 << 32), dict(max_prefix=(1 << 31) - 1),
+        dict(out=z(3, 3, 64)), dict(out=f(3, 4, 64)), dict(out=z(1, 4, 64).expand(3, 4, 64)), dict(out=z(3, 4, 66)[..., 1:65])]
+
+
+@pytest.mark.parametrize("op", ["append", "decode", "tree"])
+def test_binding_and_paged_py_refuse_alike(cuda, op, monkeypatch):
+    """What paged.py refuses, the binding leaves to it: each bad call raises the same error with and without the binding,
+    which takes none of them, and nothing is written."""
+    good, call = _base_calls(cuda)[op]
+    bind = getattr(_lib.binding(), op)
+    assert bind(*good.values()) is not NotImplemented
+    watch = (good["k_pages"].clone(), good["v_pages"].clone())
+    for i, bad in enumerate(_bad(op, cuda)):
+        kw = dict(good, **bad)
+        assert bind(*kw.values()) is NotImplemented, (i, list(bad))
+        errors = []
+        for without in (False, True):
+            with monkeypatch.context() as m:
+                if without:
+                    m.setattr(_lib, "_BINDING", _lib._NoBinding())
+                with pytest.raises((ValueError, AssertionError, _lib.CastError)) as e:
+                    call(**kw)
+                errors.append((type(e.value), str(e.value)))
+        assert errors[0] == errors[1], (i, list(bad))
+    assert torch.equal(good["k_pages"], watch[0]) and torch.equal(good["v_pages"], watch[1]) and _lib.device_error() == 0
