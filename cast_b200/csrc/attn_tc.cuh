@@ -615,8 +615,14 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
         const float alpha = rescale ? ex2(m_ref - m_tile) : 1.f;
         if (grow) m_ref = m_tile;
         const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
-        // P = exp2(S*c - m) in packed pairs (f32x2 FMA / add), 16-bit, into the first 64 columns of S
-        const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_use, -m_use);
+        // P = exp2(S*c - m) in packed pairs (f32x2 FMA / add), 16-bit, into the first 64 columns of S. One term
+        // of 16 bits (the decode kernel carries two): the second would double the P V MMAs, and this kernel is
+        // bound by tensor core and softmax, not by memory; its rounding, half a step of p, is of the size of the
+        // output's own, and the sum l takes p unrounded.
+        // Paged, half precision: P is 2^7 p (p <= 2^8), and l with it. Half precision ends at 2^-24, where a
+        // sixth of p = 1.4e-7 was lost, and below 2^-25 all of it.
+        const float up = PAGED && !BF16 ? 7.f : 0.f;
+        const float2 c2 = make_float2(c, c), nm2 = make_float2(up - m_use, up - m_use);
         float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {

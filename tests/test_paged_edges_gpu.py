@@ -400,3 +400,30 @@ def test_binding_and_paged_py_refuse_alike(cuda, op, monkeypatch):
                 errors.append((type(e.value), str(e.value)))
         assert errors[0] == errors[1], (i, list(bad))
     assert torch.equal(good["k_pages"], watch[0]) and torch.equal(good["v_pages"], watch[1]) and _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,Hq,Hkv,ps,B,n", [(128, 8, 2, 64, 40, 3000), (128, 32, 8, 16, 2, 16000), (64, 6, 2, 1, 3, 5000), (64, 4, 1, 24, 2, 900)])
+def test_tree_long_tail_of_small_probabilities(cuda, dtype, D, Hq, Hkv, ps, B, n):
+    """As for decode, over the prefix of one-token packs whose own key has the score -15.76 as well. Probabilities are one
+    16-bit term: off by half(type) of p, in half precision by half a step of its smallest, 2^-25, on 2^7 p = 2.4 x 2^-17."""
+    dt = TYPES[dtype]
+    pages = -(-n // ps)
+    at = torch.arange(pages * ps, device=cuda).view(pages, 1, ps, 1)
+    top = (at % 500 == 7).expand(pages, Hkv, ps, D)
+    level = torch.tensor(-15.76 / math.sqrt(D), dtype=dt, device=cuda)
+    k = torch.where(top, torch.zeros_like(level), level).contiguous()
+    v = torch.where(top, torch.zeros_like(level), torch.full_like(level, 1000.0)).contiguous()
+    q = torch.ones(B, Hq, D, dtype=dt, device=cuda)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda).repeat(B, 1)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    kp, vp = level.expand(B, Hkv, D).contiguous(), torch.full((B, Hkv, D), 1000.0, dtype=dt, device=cuda)
+    got = cast_b200.varlen_tree_attention_paged(q, k, v, table, kp, vp, i32(list(range(B + 1))), i32([n] * B), i32([1] * B),
+                                                parent=i32([-1] * B), max_pack=1, max_prefix=n)
+    assert _lib.device_error() == 0
+    s = level.double() * math.sqrt(D)
+    tops = len(range(7, n, 500))
+    tail = (n + 1 - tops) * torch.exp(s)
+    want = (1000.0 * tail / (tops + tail)).expand(B, Hq, D)
+    e = (D + 2) * 2 * U32 * s.abs().expand(B, Hq)
+    _check_attention(got, want, e, want, 0, dt, 2.0 ** -8 if dtype == "bf16" else 2.0 ** -25 / (2.4 * 2.0 ** -17))
