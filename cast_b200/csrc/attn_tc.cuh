@@ -285,8 +285,8 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
   const uint32_t ring = smem_u32(smem + (is_k ? SMEM_K : SMEM_V));
   const CUtensorMap* m_reg = is_k ? &tmK : &tmV;
   const CUtensorMap* m_pack = is_k ? &tmKp : &tmVp;
-  // Paged prefix: lane l copies panel l % PANELS of boxes l / PANELS, + 32 / PANELS, ...; the table entry of
-  // its first box in tile j + 1 is read while tile j is being copied.
+  // Paged prefix: lane l copies panel l % PANELS of box l / PANELS; the table entry of its box in tile j + 1 is
+  // read while tile j is being copied.
   auto page_at = [&](int n) -> int {
     return n < m.S ? p.page_table[b * p.table_stride + n / p.page_size] : -1;
   };
@@ -341,13 +341,12 @@ attn_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmQ, cons
     const int t = t_begin + j;
     if (LAYOUT == kPaged && t < nt_pre) {
       const int n0 = t * BN, boxes = (min(BN, m.S - n0) + p.box - 1) / p.box;
+      const int i = lane / PANELS, n = n0 + i * p.box;     // boxes of 8 rows or more: at most one to a lane
       int page = next_page;
-      next_page = page_at(n0 + BN + lane / PANELS * p.box);
+      next_page = page_at(n + BN);
       if (elect_one()) mbar_expect_tx(bar, boxes * p.box * (PANELS * 128));
       __syncwarp();
-      for (int i = lane / PANELS; i < boxes; i += 32 / PANELS) {
-        const int n = n0 + i * p.box;
-        if (i >= 32 / PANELS) page = page_at(n);
+      if (i < boxes) {
         if (page < 0 || page >= p.num_pages) {
           report(CAST_DEV_BAD_LAYOUT);
           page = p.num_pages;          // past the last page: the copy fills zeros

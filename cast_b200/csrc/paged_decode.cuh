@@ -363,7 +363,7 @@ struct Copier {
       pr -= p.page_size;
       ++pi;
     }
-    if (pi >= base + 32) {      // by 16 at most
+    if (pi >= base + 32) {      // by KS at most
       base += 32;
       page = ahead;
       ahead = entry(p, base + 32 + (threadIdx.x & 31));

@@ -447,7 +447,9 @@ int cast_paged_append(int n_layers, void* const* pages_kv, const void* const* ne
  * strides multiples of 16 bytes, bases 16-byte aligned. CAST_F32, CAST_BF16 or
  * CAST_F16, D 64 or 128. The lengths are not read on the host. Two launches; the
  * workspace (256-byte aligned, cast_paged_decode_workspace_size() bytes) needs no
- * initial value; its size depends on H_q / H_kv and D alone.
+ * initial value and serves one call at a time; its size depends on dtype, H_q / H_kv, D
+ * and the device's SM count, not on B or the lengths. NaN in a visible key or query
+ * gives NaN; visible values have to be finite (16-bit types: an infinity gives NaN).
  */
 int cast_paged_decode_attn(const void* q, const void* k_pages, const void* v_pages, void* out, float* lse, int dtype,
                            const int64_t* strides, const int32_t* page_table, int64_t table_stride, int max_pages,
@@ -466,8 +468,12 @@ size_t cast_paged_decode_workspace_size(int dtype, int B, int H_q, int H_kv, int
  * pages (page, head, row; keys and values alike), k_pack, v_pack, out (row, head);
  * multiples of 4 elements, page strides multiples of 16 bytes, bases 16-byte aligned.
  * CAST_BF16 / CAST_F16 with H_q / H_kv <= 128 and strides that are multiples of 8
- * run on the tensor cores, everything else (CAST_F32, exact) on the CUDA cores. Keys past prefix_len[b] in a page are never part of the result.
- * max_prefix bounds prefix_len[b] (a longer one is reported as CAST_DEV_BAD_LAYOUT).
+ * run on the tensor cores, everything else (CAST_F32, exact) on the CUDA cores. Keys
+ * past prefix_len[b] in a page, and pack rows past pack_len[b], are never part of a
+ * result, whatever they hold. Within a pack v has to be finite: a row that does not see
+ * a key still multiplies its value by 0. max_prefix bounds prefix_len[b] (a longer one is
+ * reported as CAST_DEV_BAD_LAYOUT); the keys are cut for it, so a bound far above the
+ * lengths leaves short prefixes in one chunk.
  */
 int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages, const void* k_pack,
                              const void* v_pack, void* out, int dtype, const int64_t* strides,
@@ -477,7 +483,8 @@ int cast_tree_attn_paged_fwd(const void* q, const void* k_pages, const void* v_p
                              int page_size, int H_q, int H_kv, int D, float sm_scale, int max_pack, int max_prefix,
                              void* workspace, size_t workspace_bytes, cast_stream_t stream);
 
-/* Bytes of workspace cast_tree_attn_paged_fwd needs for these sizes (0 is possible). */
+/* Bytes of workspace cast_tree_attn_paged_fwd needs for these sizes (0 is possible): the larger of
+ * its two forms' needs, since the strides, which choose the form, play no part here. */
 size_t cast_tree_attn_paged_workspace_size(int dtype, int B, int total_q, int H_q, int H_kv, int D, int max_pack,
                                            int max_prefix);
 
