@@ -427,3 +427,53 @@ def test_tree_long_tail_of_small_probabilities(cuda, dtype, D, Hq, Hkv, ps, B, n
     want = (1000.0 * tail / (tops + tail)).expand(B, Hq, D)
     e = (D + 2) * 2 * U32 * s.abs().expand(B, Hq)
     _check_attention(got, want, e, want, 0, dt, 2.0 ** -8 if dtype == "bf16" else 2.0 ** -25 / (2.4 * 2.0 ** -17))
+
+
+# ------------------------------------------------------------------------------------- graphs and streams
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_tree_and_accept_captured_and_on_two_streams(cuda, dtype):
+    """A verify pass and the append of its accepted rows, captured once with the table's capacity as the bound, replayed with
+    other lengths, packs, accepted rows and contents beside eager calls on another stream, each with its own workspace."""
+    dt = TYPES[dtype]
+    c, q, kp, vp, parents, cu = _tree_inputs(cuda, 65, [900, 33, 1500], [17, 1, 20], 8, 2, 128, 16, dt)
+    for t in c.k + c.v:
+        t.nan_to_num_(0.5, 0.5, 0.5)
+    room = int(torch.where(c.table >= 0, c.table < c.num, False).sum(1).min()) * 16       # keys every sequence has pages for
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    par, cu, P = i32(sum(parents, [])), i32(cu.tolist()), i32([17, 1, 20])
+    length, keep, acc = i32([20, 33, 5]), i32([[0, 3, 8], [0, -1, -1], [0, 5, -1]]), i32([3, 1, 2])
+    cap = c.table.shape[1] * 16
+    ws = [torch.full((64 << 20,), 255, dtype=torch.uint8, device=cuda) for _ in range(2)]
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    pages = [(c.k[0], c.v[0]), (c.k[0].clone(), c.v[0].clone())]
+
+    def step(i):
+        k, v = pages[i]
+        cast_b200.varlen_tree_attention_paged(q, k, v, c.table, kp, vp, cu, length, P, parent=par, max_pack=20, max_prefix=cap,
+                                              out=outs[i], workspace=ws[i])
+        cast_b200.append_paged(k, v, c.table, length, kp, vp, cu, keep=keep, accepted=acc)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(0)
+    g = torch.Generator(device=cuda).manual_seed(66)
+    for lens, took in (([20, 33, 5], [3, 1, 2]), ([0, 1, 40], [0, 1, 1]), ([room - 3, 17, 16], [3, 0, 2])):
+        length.copy_(i32(lens))
+        acc.copy_(i32(took))
+        q.normal_(generator=g)
+        pages[0][0].normal_(generator=g)
+        pages[1][0].copy_(pages[0][0])
+        pages[1][1].copy_(pages[0][1])
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            step(1)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(outs[0], outs[1]) and torch.isfinite(outs[0]).all()
+        assert torch.equal(pages[0][0], pages[1][0]) and torch.equal(pages[0][1], pages[1][1])
+    assert _lib.device_error() == 0
