@@ -18,7 +18,8 @@ and a verify round of draft trees, whose accepted rows are appended for every la
     append_paged(all_k_pages, all_v_pages, table, length, all_k_packs, all_v_packs, cu_q, keep=walk.keep,
                  accepted=walk.accepted)
 
-A length or page id out of range is skipped on the device and reported by ``_lib.device_error()``.
+A length or page id out of range is skipped on the device and reported by ``_lib.device_error()``; the results of that
+sequence are undefined. A workspace serves one call at a time.
 
 Each call first goes to the binding (``csrc/paged_binding.cpp``), which takes arguments that are already as the C ABI
 wants them; everything else (conversions, copies, refusals) is done here.
@@ -312,8 +313,9 @@ def varlen_tree_attention_paged(q, k_pages, v_pages, page_table, k_pack, v_pack,
     q: [total_q, H_q, D]; request b's prefix is keys [0, prefix_len[b]) of its pages; k_pack / v_pack:
     [total_q, H_kv, D], this pass's keys and values in pack order. Output, masks and conventions as
     varlen_tree_attention. bfloat16 / float16 with H_q / H_kv <= 128 run on the tensor cores straight from the
-    pages, whatever their size; float32 on the exact CUDA-core kernel. D 64 or 128.
-    max_pack / max_prefix bound pack_len and prefix_len; given, the call reads nothing back to the host.
+    pages, whatever their size; float32 on the exact CUDA-core kernel (the store form's fp32_path="exact"; its split path
+    has no form on pages). D 64 or 128. max_pack / max_prefix bound pack_len and prefix_len; given, the call reads nothing
+    back to the host. The keys are split for max_prefix: a bound far above the lengths costs short prefixes time.
     """
     done = (_lib._BINDING or _lib.binding()).tree(q, k_pages, v_pages, page_table, k_pack, v_pack, cu_q, prefix_len,
                                                   pack_len, ancestor_mask, sm_scale, parent, max_pack, max_prefix, out,
